@@ -452,6 +452,19 @@ int mlc_encode_embedding_q4_0(mlc_ctx* ctx, const void* table, size_t row_stride
  * vocab logits. group_rows = 0 or >= vocab: logits is a plain [batch, vocab] array; otherwise the walker's
  * layout, groups of group_rows vocabulary rows, each group a [batch, rows of the group] array. */
 int mlc_encode_argmax_rows(mlc_ctx* ctx, const void* logits, size_t batch, size_t vocab, size_t group_rows, void* out_ids);
+/* One selection step of beam search on the device, beside the argmax above. logits holds groups * beams
+ * rows (row g * beams + p = beam p of group g), laid out as for mlc_encode_argmax_rows; cum_scores device fp32
+ * [groups, beams]. With x the logits of a row,
+ *   score(p, t) = cum_scores[g, p] + x[t] - log sum_u exp x[u],
+ * and the n_select best (p, t) of every group go to out_scores (fp32), out_parents (uint32 p) and out_tokens
+ * (uint32 t), each [groups, n_select], best first; equal scores: the lower p, then the lower t. finished (device
+ * uint8 [groups, beams], may be NULL): a beam with a nonzero entry has one candidate, (p, pad_token) with its score
+ * as it is, and its logits are not read. Candidates whose score is -inf or not a number (a logit of -inf or NaN, a row
+ * with a +inf) are never selected; places that stay empty get -inf and 0xFFFFFFFF. beams and n_select <= 64
+ * (MLC_ERR_UNSUPPORTED). Capturable once the call has run outside a capture. */
+int mlc_encode_beam_select(mlc_ctx* ctx, const void* logits, const void* cum_scores, const void* finished, size_t groups,
+                           size_t beams, size_t vocab, size_t group_rows, size_t n_select, uint32_t pad_token,
+                           void* out_scores, void* out_parents, void* out_tokens);
 /* The same mat-vec with its neighbours in the walker fused in (no counterpart in the reference).
  * input_kind 0: in = fp32 [batch, in_stride], as above.
  * input_kind 1: the input row n is SiLU(in[n, c]) * in[n, cols + c], computed on load (in = the
@@ -508,6 +521,89 @@ int mlc_encode_paged_prefill_attention(mlc_ctx* ctx, const void* q, const void* 
                                        size_t num_heads, size_t kv_heads, size_t head_dim,
                                        size_t page_size_tokens, float scale, int q_dtype, int o_dtype,
                                        size_t capacity_pages);
+
+/* ---- attention for a tree of drafted tokens over the cache -----------------------------
+ * No counterpart in the reference, which decodes one continuation per request. A request has
+ * prefix_lens[r] committed tokens in its pages and draft_lens[r] drafted tokens whose K/V rows sit
+ * behind them, drafted token i at position prefix_lens[r] + i (scatter them first, e.g. with
+ * mlc_encode_scatter_kv_pair_paged_batched_f16). One call computes the attention of all drafted
+ * tokens of all requests:
+ *   O[i,h,:] = sum_s w_s V[s,kv_h,:] / sum_s w_s,  w_s = exp(scale * Q[i,h,:].K[s,kv_h,:]),
+ * s over every committed token and the drafted tokens j whose bit is set in token i's mask row. A
+ * row whose mask and prefix leave nothing (or whose visible scores are all -inf) gives zeros. What
+ * lies in rows that a token does not see - other branches, slots behind the last token - has no
+ * effect on it, infinities and NaN included.
+ *   q, o          device [sum_r draft_lens[r], num_heads, head_dim], request after request, fp16 or
+ *                 fp32 per q_dtype / o_dtype
+ *   tree_mask     host u32 [sum_r draft_lens[r], mask_words]: bit j of row i (word j / 32, bit
+ *                 j % 32) set = drafted token i sees drafted token j of its request. A tree sets a
+ *                 token's own bit and its ancestors'. Bits at or above draft_lens[r] are ignored;
+ *                 mask_words * 32 must be >= every draft_lens[r].
+ *   the other tables, scale, capacity_pages as in mlc_encode_paged_flash_attention;
+ *   prefix_lens[r] + draft_lens[r] must fit the request's pages. Requests without drafted tokens
+ *   are allowed.
+ * run_: validates, launches, waits. encode_: asynchronous, needs an open pass. The plan keeps one
+ * pass's tables on the device for the calls of all its layers (and for capture into a graph):
+ * update replaces them in stream order; a plan that a captured graph uses can no longer be updated
+ * (MLC_ERR_UNSUPPORTED) and must outlive that graph. A plan belongs to the context that made it. */
+typedef struct mlc_tree_plan mlc_tree_plan;
+int mlc_run_paged_tree_attention(mlc_ctx* ctx, const void* q, const void* k_pages, const void* v_pages, void* o,
+                                 const uint32_t* page_tables_flat, size_t n_page_tables_flat,
+                                 const uint32_t* page_table_offsets, const uint32_t* prefix_lens,
+                                 const uint32_t* draft_lens, const uint32_t* tree_mask, size_t mask_words, size_t batch,
+                                 size_t num_heads, size_t kv_heads, size_t head_dim, size_t page_size_tokens,
+                                 float scale, int q_dtype, int o_dtype, size_t capacity_pages);
+int mlc_encode_paged_tree_attention(mlc_ctx* ctx, const void* q, const void* k_pages, const void* v_pages, void* o,
+                                    const uint32_t* page_tables_flat, size_t n_page_tables_flat,
+                                    const uint32_t* page_table_offsets, const uint32_t* prefix_lens,
+                                    const uint32_t* draft_lens, const uint32_t* tree_mask, size_t mask_words,
+                                    size_t batch, size_t num_heads, size_t kv_heads, size_t head_dim,
+                                    size_t page_size_tokens, float scale, int q_dtype, int o_dtype,
+                                    size_t capacity_pages);
+int mlc_tree_plan_create(mlc_ctx* ctx, const uint32_t* page_tables_flat, size_t n_page_tables_flat,
+                         const uint32_t* page_table_offsets, const uint32_t* prefix_lens, const uint32_t* draft_lens,
+                         const uint32_t* tree_mask, size_t mask_words, size_t batch, size_t num_heads, size_t kv_heads,
+                         size_t head_dim, size_t page_size_tokens, size_t capacity_pages, mlc_tree_plan** out);
+int mlc_tree_plan_update(mlc_ctx* ctx, mlc_tree_plan* plan, const uint32_t* page_tables_flat, size_t n_page_tables_flat,
+                         const uint32_t* page_table_offsets, const uint32_t* prefix_lens, const uint32_t* draft_lens,
+                         const uint32_t* tree_mask, size_t mask_words, size_t batch);
+void mlc_tree_plan_destroy(mlc_ctx* ctx, mlc_tree_plan* plan);
+int mlc_encode_paged_tree_attention_planned(mlc_ctx* ctx, const mlc_tree_plan* plan, const void* q, const void* k_pages,
+                                            const void* v_pages, void* o, float scale, int q_dtype, int o_dtype);
+
+/* ---- copies inside the pools: forked requests, accepted drafts ------------------------------
+ * No counterpart in the reference, whose requests own their pages for good. pools: host array of
+ * n_pools device pointers, as a rule the K and V pools of every layer - one launch moves the same
+ * pages or rows in all of them. Each pool may be named once; pools must not overlap. Elements of
+ * dtype_bytes (2 or 4). run_ waits, encode_ needs an open pass; both take host tables and are not
+ * capturable.
+ *
+ * copy_kv_pages: page dst_page_ids[i] becomes a copy of page src_page_ids[i], whole pages, bit for
+ * bit. One page may go to several destinations; a destination named twice, or one that is also the
+ * source of another pair, is MLC_ERR_INVALID_ARG (the copies run side by side). src == dst is
+ * allowed and does nothing. */
+int mlc_run_copy_kv_pages(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* src_page_ids,
+                          const uint32_t* dst_page_ids, size_t n_pairs, size_t page_size_tokens, size_t n_kv_heads,
+                          size_t head_dim, size_t dtype_bytes, size_t capacity_pages);
+int mlc_encode_copy_kv_pages(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* src_page_ids,
+                             const uint32_t* dst_page_ids, size_t n_pairs, size_t page_size_tokens, size_t n_kv_heads,
+                             size_t head_dim, size_t dtype_bytes, size_t capacity_pages);
+/* compact_kv_rows: the rows of accepted drafted tokens move up behind the committed ones. For
+ * request r the rows at positions start_positions[r] + kept_rows[kept_offsets[r] + i] go to
+ * positions start_positions[r] + i, as if every source were read before any destination is
+ * written. A request's kept rows must rise strictly (MLC_ERR_INVALID_ARG) and lie inside its pages
+ * (MLC_ERR_BOUNDS). Rows behind the last kept one keep their bytes. Two requests must not touch
+ * the same page where rows move (MLC_ERR_INVALID_ARG: copy a shared page first). */
+int mlc_run_compact_kv_rows(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* page_tables_flat,
+                            size_t n_page_tables_flat, const uint32_t* page_table_offsets,
+                            const uint32_t* start_positions, const uint32_t* kept_rows, const uint32_t* kept_offsets,
+                            size_t batch, size_t page_size_tokens, size_t n_kv_heads, size_t head_dim,
+                            size_t dtype_bytes, size_t capacity_pages);
+int mlc_encode_compact_kv_rows(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* page_tables_flat,
+                               size_t n_page_tables_flat, const uint32_t* page_table_offsets,
+                               const uint32_t* start_positions, const uint32_t* kept_rows, const uint32_t* kept_offsets,
+                               size_t batch, size_t page_size_tokens, size_t n_kv_heads, size_t head_dim,
+                               size_t dtype_bytes, size_t capacity_pages);
 
 /* ---- split-KV across GPUs without a collective library: peer-memory exchange + combine --
  * One kernel per step and rank: it stores this rank's (o, m, l) partial into every rank's

@@ -83,6 +83,22 @@ _PROTOTYPES = {
     "mlc_encode_matmul_quant_fused": (_i, [_vp, _i, _vp, _vp, _sz, _i, _vp, _sz, _sz, _sz, _sz, _vp]),
     "mlc_encode_argmax_rows": (_i, [_vp, _vp, _sz, _sz, _sz, _vp]),
     "mlc_encode_matmul_gate_up_silu_packed": (_i, [_vp, _i, _vp, _vp, _sz, _i, _sz, _sz, _sz, _sz, _vp]),
+    "mlc_encode_beam_select": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.c_uint32, _vp, _vp, _vp]),
+    "mlc_run_paged_tree_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz,
+                                          _sz, _sz, _sz, _f, _i, _i, _sz]),
+    "mlc_encode_paged_tree_attention": (_i, [_vp, _vp, _vp, _vp, _vp, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz,
+                                             _sz, _sz, _sz, _sz, _f, _i, _i, _sz]),
+    "mlc_tree_plan_create": (_i, [_vp, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz, _sz, _sz, _sz, _sz,
+                                  C.POINTER(_vp)]),
+    "mlc_tree_plan_update": (_i, [_vp, _vp, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz]),
+    "mlc_tree_plan_destroy": (None, [_vp, _vp]),
+    "mlc_encode_paged_tree_attention_planned": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i]),
+    "mlc_run_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _u32p, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "mlc_encode_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _u32p, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "mlc_run_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz, _sz,
+                                     _sz, _sz]),
+    "mlc_encode_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz,
+                                        _sz, _sz, _sz]),
     "mlc_compute_rotary_coefficients": (_i, [_sz, _sz, _f, _f, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "mlc_exchange_create": (_i, [_vp, _i, _i, _sz, _sz, C.POINTER(_vp)]),
     "mlc_exchange_handle": (_i, [_vp, _vp, _vp]),
@@ -552,6 +568,129 @@ class Executor:
         return self.status(self._lib.mlc_encode_lse_combine(
             self._h, _vp(_ptr(o_parts)), _vp(_ptr(ml_parts)), parts, rows, head_dim, _vp(_ptr(out)), o_dtype))
 
+    # -- several continuations of one request: tree attention, page copies, beam selection --------
+    @staticmethod
+    def _treeTables(page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask, batch):
+        flat, pflat = _u32(page_tables_flat)
+        off, poff = _u32(page_table_offsets)
+        pre, ppre = _u32(prefix_lens)
+        dr, pdr = _u32(draft_lens)
+        mask, pmask = _u32(tree_mask)
+        if off.size != batch + 1 or pre.size != batch or dr.size != batch or mask.ndim != 2 or mask.shape[0] != int(dr.sum()):
+            return None
+        return (flat, off, pre, dr, mask), (pflat, flat.size, poff, ppre, pdr, pmask, mask.shape[1])
+
+    def _tree(self, fn, q, k_pages, v_pages, o, page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask,
+              batch, num_heads, kv_heads, head_dim, page_size_tokens, scale, q_dtype, o_dtype, capacity_pages) -> bool:
+        t = self._treeTables(page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask, batch)
+        if t is None:
+            return self.status(1)
+        return self.status(fn(self._h, _vp(_ptr(q)), _vp(_ptr(k_pages)), _vp(_ptr(v_pages)), _vp(_ptr(o)), *t[1], batch,
+                              num_heads, kv_heads, head_dim, page_size_tokens, float(scale), q_dtype, o_dtype,
+                              capacity_pages))
+
+    def runPagedTreeAttention(self, q, k_pages, v_pages, o, page_tables_flat, page_table_offsets, prefix_lens, draft_lens,
+                              tree_mask, batch, num_heads, kv_heads, head_dim, page_size_tokens, scale: float = 0.0,
+                              q_dtype: int = MLC_F16, o_dtype: int = MLC_F16, capacity_pages: int = 0) -> bool:
+        """Attention of all requests' drafted tokens over committed tokens and, by tree_mask (uint32
+        [sum(draft_lens), mask_words], bit j of row i = token i sees drafted token j), each other.
+        q / o are [sum(draft_lens), num_heads, head_dim]; treeMask() builds the mask from parent indices."""
+        return self._tree(self._lib.mlc_run_paged_tree_attention, q, k_pages, v_pages, o, page_tables_flat,
+                          page_table_offsets, prefix_lens, draft_lens, tree_mask, batch, num_heads, kv_heads, head_dim,
+                          page_size_tokens, scale, q_dtype, o_dtype, capacity_pages)
+
+    def encodePagedTreeAttention(self, q, k_pages, v_pages, o, page_tables_flat, page_table_offsets, prefix_lens, draft_lens,
+                                 tree_mask, batch, num_heads, kv_heads, head_dim, page_size_tokens, scale: float = 0.0,
+                                 q_dtype: int = MLC_F16, o_dtype: int = MLC_F16, capacity_pages: int = 0) -> bool:
+        return self._tree(self._lib.mlc_encode_paged_tree_attention, q, k_pages, v_pages, o, page_tables_flat,
+                          page_table_offsets, prefix_lens, draft_lens, tree_mask, batch, num_heads, kv_heads, head_dim,
+                          page_size_tokens, scale, q_dtype, o_dtype, capacity_pages)
+
+    @staticmethod
+    def treeMask(parents) -> np.ndarray:
+        """Mask rows of drafted trees: parents is a list with, per request, each drafted token's parent (an index
+        below its own, or -1 for a child of the last committed token). Returns uint32 [sum of lengths, words]."""
+        words = max(1, max((len(p) + 31) // 32 for p in parents)) if len(parents) else 1
+        rows = np.zeros((sum(len(p) for p in parents), words), np.uint32)
+        first = 0
+        for p in parents:
+            for i, parent in enumerate(p):
+                if not -1 <= parent < i:
+                    raise ValueError("a drafted token's parent comes before it")
+                if parent >= 0:
+                    rows[first + i] = rows[first + parent]
+                rows[first + i, i // 32] |= np.uint32(1 << (i % 32))
+            first += len(p)
+        return rows
+
+    def createTreePlan(self, page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask, batch, num_heads,
+                       kv_heads, head_dim, page_size_tokens, capacity_pages=0) -> "TreePlan":
+        t = self._treeTables(page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask, batch)
+        if t is None:
+            raise MlcError(1, "table sizes do not match batch")
+        h = _vp()
+        self.check(self._lib.mlc_tree_plan_create(self._h, *t[1], batch, num_heads, kv_heads, head_dim, page_size_tokens,
+                                                  capacity_pages, C.byref(h)))
+        return TreePlan(self, h)
+
+    def encodePagedTreeAttentionPlanned(self, plan, q, k_pages, v_pages, o, scale=0.0, q_dtype=MLC_F16,
+                                        o_dtype=MLC_F16) -> bool:
+        return self.status(self._lib.mlc_encode_paged_tree_attention_planned(
+            self._h, plan.handle, _ptr(q), _ptr(k_pages), _ptr(v_pages), _ptr(o), scale, q_dtype, o_dtype))
+
+    def _copyPages(self, fn, pools, src_page_ids, dst_page_ids, page_size_tokens, n_kv_heads, head_dim, dtype_bytes,
+                   capacity_pages) -> bool:
+        src, psrc = _u32(src_page_ids)
+        dst, pdst = _u32(dst_page_ids)
+        if src.size != dst.size:
+            return self.status(1)
+        return self.status(fn(self._h, pools, len(pools), psrc, pdst, src.size, page_size_tokens, n_kv_heads, head_dim,
+                              dtype_bytes, capacity_pages))
+
+    def copyKVPages(self, pools, src_page_ids, dst_page_ids, page_size_tokens, n_kv_heads, head_dim, dtype_bytes=2,
+                    capacity_pages: int = 0) -> bool:
+        """Whole pages inside every pool of `pools` (a pointerArray), one launch."""
+        return self._copyPages(self._lib.mlc_run_copy_kv_pages, pools, src_page_ids, dst_page_ids, page_size_tokens,
+                               n_kv_heads, head_dim, dtype_bytes, capacity_pages)
+
+    def encodeCopyKVPages(self, pools, src_page_ids, dst_page_ids, page_size_tokens, n_kv_heads, head_dim, dtype_bytes=2,
+                          capacity_pages: int = 0) -> bool:
+        return self._copyPages(self._lib.mlc_encode_copy_kv_pages, pools, src_page_ids, dst_page_ids, page_size_tokens,
+                               n_kv_heads, head_dim, dtype_bytes, capacity_pages)
+
+    def _compactRows(self, fn, pools, page_tables_flat, page_table_offsets, start_positions, kept_rows, kept_offsets, batch,
+                     page_size_tokens, n_kv_heads, head_dim, dtype_bytes, capacity_pages) -> bool:
+        flat, pflat = _u32(page_tables_flat)
+        off, poff = _u32(page_table_offsets)
+        start, pstart = _u32(start_positions)
+        kept, pkept = _u32(kept_rows)
+        koff, pkoff = _u32(kept_offsets)
+        if off.size != batch + 1 or start.size != batch or koff.size != batch + 1 or kept.size < int(koff[-1]):
+            return self.status(1)
+        return self.status(fn(self._h, pools, len(pools), pflat, flat.size, poff, pstart, pkept, pkoff, batch,
+                              page_size_tokens, n_kv_heads, head_dim, dtype_bytes, capacity_pages))
+
+    def compactKVRows(self, pools, page_tables_flat, page_table_offsets, start_positions, kept_rows, kept_offsets, batch,
+                      page_size_tokens, n_kv_heads, head_dim, dtype_bytes=2, capacity_pages: int = 0) -> bool:
+        """Rows start_positions[r] + kept_rows[...] of request r move to start_positions[r] + 0, 1, 2, ... in
+        every pool of `pools` (a pointerArray), one launch."""
+        return self._compactRows(self._lib.mlc_run_compact_kv_rows, pools, page_tables_flat, page_table_offsets,
+                                 start_positions, kept_rows, kept_offsets, batch, page_size_tokens, n_kv_heads, head_dim,
+                                 dtype_bytes, capacity_pages)
+
+    def encodeCompactKVRows(self, pools, page_tables_flat, page_table_offsets, start_positions, kept_rows, kept_offsets,
+                            batch, page_size_tokens, n_kv_heads, head_dim, dtype_bytes=2, capacity_pages: int = 0) -> bool:
+        return self._compactRows(self._lib.mlc_encode_compact_kv_rows, pools, page_tables_flat, page_table_offsets,
+                                 start_positions, kept_rows, kept_offsets, batch, page_size_tokens, n_kv_heads, head_dim,
+                                 dtype_bytes, capacity_pages)
+
+    def encodeBeamSelect(self, logits, cum_scores, finished, groups, beams, vocab, group_rows, n_select, pad_token,
+                         out_scores, out_parents, out_tokens) -> bool:
+        """The n_select best (beam, token) of every group by cum_scores + log softmax(logits); finished may be None."""
+        return self.status(self._lib.mlc_encode_beam_select(
+            self._h, _ptr(logits), _ptr(cum_scores), _ptr(finished), groups, beams, vocab, group_rows, n_select, pad_token,
+            _ptr(out_scores), _ptr(out_parents), _ptr(out_tokens)))
+
     # -- CUDA graphs -------------------------------------------------------------------
     def beginCapture(self) -> bool:
         return self.status(self._lib.mlc_graph_begin_capture(self._h))
@@ -586,6 +725,32 @@ class Plan:
     def destroy(self):
         if self.handle and self._ex._h:
             self._ex._lib.mlc_attn_plan_destroy(self._ex._h, self.handle)
+        self.handle = None
+
+    def __del__(self):
+        try:
+            self.destroy()
+        except Exception:
+            pass
+
+
+class TreePlan:
+    """Tables of one pass of tree attention on the device (createTreePlan)."""
+
+    def __init__(self, ex: Executor, handle):
+        self._ex, self.handle = ex, handle
+
+    def update(self, page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask) -> bool:
+        """The next pass's tables into the same plan; its buffers are reused."""
+        batch = len(prefix_lens)
+        t = Executor._treeTables(page_tables_flat, page_table_offsets, prefix_lens, draft_lens, tree_mask, batch)
+        if t is None:
+            return self._ex.status(1)
+        return self._ex.status(self._ex._lib.mlc_tree_plan_update(self._ex._h, self.handle, *t[1], batch))
+
+    def destroy(self):
+        if self.handle and self._ex._h:
+            self._ex._lib.mlc_tree_plan_destroy(self._ex._h, self.handle)
         self.handle = None
 
     def __del__(self):

@@ -6,6 +6,7 @@
 // the reference maps onto one Metal command buffer and that maps here onto one
 // CUDA stream.
 #include "ctx.hpp"
+#include "op_util.hpp"
 
 #include <cstdlib>
 #include <cstring>
@@ -99,8 +100,42 @@ int ensure_workspace(mlc_ctx* ctx, size_t bytes, size_t counters) {
     return MLC_OK;
 }
 
+int ensure_op_scratch(mlc_ctx* ctx, OpScratch& s, size_t bytes, const char* what) {
+    if (bytes <= s.bytes) return MLC_OK;
+    if (ctx->capturing) return ctx->fail(MLC_ERR_UNSUPPORTED, "%s must grow: run the step once outside the capture first", what);
+    s.retired.reserve(s.retired.size() + 1);
+    const size_t want = bytes + bytes / 2;
+    void* p = nullptr;
+    if (cudaMalloc(&p, want) != cudaSuccess) {
+        cudaGetLastError();
+        return ctx->fail(MLC_ERR_OOM, "%s of %zu bytes unavailable", what, want);
+    }
+    if (cudaMemsetAsync(p, 0, want, ctx->stream) != cudaSuccess) {
+        cudaFree(p);
+        return ctx->fail(MLC_ERR_CUDA, "%s could not be cleared", what);
+    }
+    if (s.dev) s.retired.push_back(s.dev);
+    s.dev = p;
+    s.bytes = want;
+    ++ctx->allocations;
+    return MLC_OK;
+}
+
+static void free_op_scratch(OpScratch& s) {
+    for (void* p : s.retired) cudaFree(p);
+    if (s.dev) cudaFree(s.dev);
+    s = OpScratch();
+}
+
+void note_pool_writes(mlc_ctx* ctx, void* const* pools, size_t n_pools) {
+    std::swap(ctx->recent_writes[0], ctx->recent_writes[1]);   // the lists keep their storage
+    ctx->recent_writes[1].few[0] = ctx->recent_writes[1].few[1] = nullptr;
+    ctx->recent_writes[1].many.assign(pools, pools + n_pools);
+}
+
 void reset_after_device_error(mlc_ctx* ctx) {
     cudaMemset(ctx->d_err, 0, 4);
+    if (ctx->beam_counters.dev) cudaMemset(ctx->beam_counters.dev, 0, ctx->beam_counters.bytes);
     if (ctx->d_counters && ctx->n_counters) cudaMemset(ctx->d_counters, 0, ctx->n_counters * 4);
     for (uint32_t* block : ctx->ext_counter_block)
         if (block) cudaMemset(block, 0, kExtCounterBytes);
@@ -186,6 +221,9 @@ void mlc_ctx_destroy(mlc_ctx* ctx) {
     }
     if (ctx->d_work) cudaFree(ctx->d_work);
     if (ctx->d_counters) cudaFree(ctx->d_counters);
+    free_op_scratch(ctx->tree_scratch);
+    free_op_scratch(ctx->beam_scratch);
+    free_op_scratch(ctx->beam_counters);
     if (ctx->d_err) cudaFree(ctx->d_err);
     if (ctx->h_err) cudaFreeHost(ctx->h_err);
     if (ctx->d_trace) cudaFree(ctx->d_trace);

@@ -47,6 +47,13 @@ struct ExchangeView {
     uint32_t rank = 0, world = 1;
 };
 
+// Device scratch that outlives growth (op_util.hpp).
+struct OpScratch {
+    void* dev = nullptr;
+    size_t bytes = 0;
+    std::vector<void*> retired;
+};
+
 struct AttnPlanCache;  // attn_api.cu
 struct TensorMapCache; // attn_decode_tma.cu
 
@@ -93,6 +100,10 @@ struct mlc_ctx {
     size_t trace_words = 0;
     uint32_t trace_ctas = 0;
     uint32_t trace_parity = 0;  // which half of d_trace the most recent launch wrote
+    // scratch of tree attention's partials and of beam selection's per-chunk candidates (op_util.hpp)
+    mlcb::OpScratch tree_scratch, beam_scratch, beam_counters;
+    std::vector<uint64_t> page_marks;   // per page id: the call that last named it, and for whom (kv_pages.cu)
+    uint64_t page_mark = 0;
     mlcb::AttnPlanCache* plan_cache = nullptr;
     mlcb::TensorMapCache* tmap_cache = nullptr;
     void* tmap_encode_fn = nullptr;  // cuTensorMapEncodeTiled, resolved through the runtime

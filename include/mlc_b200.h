@@ -200,7 +200,7 @@ int mlc_encode_paged_flash_attention(mlc_ctx* ctx, const void* q, const void* k_
  * otherwise the general kernel), 1 = always the general kernel. Both are CUDA. */
 int mlc_ctx_set_attention_kernel(mlc_ctx* ctx, int which);
 /* Which family the most recent attention call used: 0 none yet, 1 general, 2 TMA decode,
- * 3 tcgen05 chunked prefill. */
+ * 3 tcgen05 chunked prefill, 4 tcgen05 tree attention. */
 int mlc_ctx_last_attention_kernel(const mlc_ctx* ctx);
 
 /* ---- device-resident plans --------------------------------------------------------

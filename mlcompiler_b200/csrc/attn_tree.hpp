@@ -72,13 +72,17 @@ struct TreeArgs {
     int q_dtype = MLC_F16, o_dtype = MLC_F16;
 };
 
-// Whether the tensor-core kernel takes this shape.
+// Whether the tensor-core kernel takes this shape: head_dim 64 or 128, pages of 16, 32 or a multiple of 64 tokens, a pool of
+// known size; and these buffers.
 bool tree_tcgen05_shape(const TreeShape& s);
-// CTAs of it that an SM holds at a time.
-uint32_t tree_tcgen05_ctas_per_sm(const TreeShape& s);
+bool tree_tcgen05_buffers(const TreeArgs& a);
+static constexpr uint32_t kTreeCtasPerSm = 2;
 // Cuts the units of a call into pieces for `max_ctas` CTAs (host arithmetic only).
 void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, TreeWork* out);
+// Device scratch for the partials of cut units.
+size_t tree_scratch_bytes(const TreeShape& s, uint32_t n_slots, uint32_t slot_rows);
 
+int launch_tree_tcgen05(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a);
 int launch_tree_general(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a);
 
 }  // namespace mlcb

@@ -153,8 +153,19 @@ int check_call(mlc_ctx* ctx, const TreeArgs& a) {
 int launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, TreeArgs a) {
     if (s.tokens == 0) return MLC_OK;
     if (!(a.scale > 0.f)) a.scale = 1.0f / std::sqrt(static_cast<float>(s.D));
+    if (v.n_cta && !ctx->force_general && tree_tcgen05_buffers(a)) {
+        ctx->last_attention_kernel = 4;
+        return launch_tree_tcgen05(ctx, s, v, a);
+    }
     ctx->last_attention_kernel = 1;
     return launch_tree_general(ctx, s, v, a);
+}
+
+// The work list of the tensor-core kernel, and room for its partials.
+int prepare_work(mlc_ctx* ctx, const TreeShape& s, const TreeTables& t, TreeWork* w) {
+    if (!tree_tcgen05_shape(s)) return MLC_OK;
+    tree_work_list(s, t, static_cast<uint32_t>(ctx->sm_count) * kTreeCtasPerSm, w);
+    return ensure_op_scratch(ctx, ctx->tree_scratch, tree_scratch_bytes(s, w->n_slots, w->slot_rows), "tree attention scratch");
 }
 
 // One call with host tables: the image goes through the context's staging area.
@@ -170,6 +181,7 @@ int tree_impl(mlc_ctx* ctx, bool sync, const TreeArgs& a, TreeShape s, const Tre
     if (s.tokens == 0) return MLC_OK;
     DeviceGuard guard(ctx->device);
     TreeWork w;
+    if ((st = prepare_work(ctx, s, t, &w)) != MLC_OK) return st;
     const TreeLayout l = layout_of(s, w);
     void *h = nullptr, *d = nullptr;
     if (!stage_reserve(ctx, l.total, &h, &d)) return MLC_ERR_OOM;
@@ -203,9 +215,10 @@ int fill_plan(mlc_ctx* ctx, mlc_tree_plan& p, TreeShape s, const TreeTables& t, 
     int st = check_tables(s, t, n_flat, &why);
     if (st != MLC_OK) return ctx->fail(st, "%s", why.c_str());
     if (ctx->capturing) return ctx->fail(MLC_ERR_UNSUPPORTED, "new tables inside a graph capture: create the plan before capturing");
-    TreeWork w;
-    const TreeLayout l = layout_of(s, w);
     DeviceGuard guard(ctx->device);
+    TreeWork w;
+    if ((st = prepare_work(ctx, s, t, &w)) != MLC_OK) return st;
+    const TreeLayout l = layout_of(s, w);
     if (!p.uploaded) MLCB_CUDA(ctx, cudaEventCreateWithFlags(&p.uploaded, cudaEventDisableTiming));
     if (l.total > p.cap) {
         const size_t want = l.total + l.total / 2;

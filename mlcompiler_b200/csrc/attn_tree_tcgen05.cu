@@ -1,0 +1,767 @@
+// Attention of drafted tokens over the paged cache on the 5th-generation tensor cores: tcgen05.mma with accumulators
+// in tensor memory, K and V staged by TMA.
+//
+// The rows that share a KV head - G heads of every drafted token of a request - are one operand: with 16 drafted
+// tokens and a group of 8 they fill the 128 rows of the tensor core's tile, and every K / V tile is read once for all of
+// them. Per 64 tokens of the cache:
+//   S[128x64]  = Q[128xD] . K^T       A and B from shared memory, fp32 accumulator in tensor memory
+//   softmax    : thread t owns row t; running maximum and sum in fp32, base-2 exponentials, P rounded to fp16 back into
+//                tensor memory as the next A operand. The output is rescaled only when a row's maximum has grown by
+//                more than 2^8 since the last rescale (exact: P <= 256, and the final 1 / l uses the same reference)
+//   O[128xD] += P[128x64] . V
+// The tree mask only matters in the tiles that hold drafted tokens, the last ones of a request: there a row's 64 mask
+// bits are cut out of its mask words. In those tiles V is also searched for infinities and NaN - a masked token has
+// weight 0, and 0 * inf would reach rows that do not see it; they are replaced by 0, and added at the end to the rows
+// that do see them.
+//
+// fp32 queries or outputs (EXACT): an fp16 operand carries 11 bits, so Q (scaled by a power of two per row) and P enter as
+// two fp16 halves, two products each: 22 bits of each, K and V are fp16 as they are.
+//
+// What bounds it: the cache is read once, 4 * rows flop per byte - memory up to about 128 rows, the exponentials and the
+// tensor core's issue above. The cache tiles of all (request, KV head, row tile) units are dealt evenly to a resident
+// grid (attn_tree_plan.cpp); units cut between CTAs leave un-normalised partials that tree_merge_kernel joins, launched as
+// a programmatic dependent.
+//
+// Warps 0-3: softmax and output (warp w reads tensor-memory lanes 32w..32w+31), warp 4: MMA issue, warps 5 / 6: TMA
+// producers of K / V. S is double-buffered so that Q.K^T of tile j+1 runs under the softmax of tile j. No cluster.
+#include <cuda.h>
+#include <cuda_fp16.h>
+
+#include "attn_tree.hpp"
+#include "op_util.hpp"
+#include "tcgen05_util.hpp"
+
+namespace mlcb {
+
+namespace {
+
+constexpr uint32_t kSlabQ = kTreeRows * 128;   // 64 halfs of every query row
+constexpr uint32_t kSlabKV = kTreeTile * 128;  // 64 halfs of every token of a tile
+constexpr uint32_t kTmemCols = 256;            // O: up to 128 columns, S: 2 x 64
+constexpr uint32_t kTmemS = 128;
+constexpr uint32_t kThreads = 224;
+
+template <int D, bool EXACT>
+struct Config {
+    static constexpr uint32_t slabs = D / 64;
+    static constexpr uint32_t q_bytes = slabs * kSlabQ * (EXACT ? 2 : 1);
+    static constexpr uint32_t kv_bytes = slabs * kSlabKV;   // one tile of K, or of V
+    // two CTAs per SM share 226 KB; with D = 128 the two halves of Q leave room for one CTA only
+    static constexpr uint32_t ctas = EXACT && D == 128 ? 1 : 2;
+    static constexpr uint32_t stages = EXACT ? 4 : (D == 128 ? 2 : 5);
+    static constexpr uint32_t tile_bytes = q_bytes + stages * 2 * kv_bytes;
+};
+
+template <uint32_t STAGES>
+struct Bars {
+    uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done;
+    uint32_t tmem_slot, not_finite;
+};
+
+struct TreeParams {
+    const void* q;
+    const __half* v_pages;
+    void* o;
+    float* part_o;    // [slot][slot_rows][D]
+    float2* part_ml;  // [slot][slot_rows] (reference maximum in base-2 units, sum)
+    const TreePiece* pieces;
+    const uint32_t *cta_off, *pt_flat, *mask;
+    uint32_t* err;
+    uint32_t H, KVH, G, P, mask_words, slot_rows;
+    uint32_t box_rows, boxes;   // TMA boxes of a tile: boxes * box_rows = 64
+    float scale_log2;
+    int q_f32, o_f32;
+};
+
+using tc::smem_u32;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
+// A poll that finds the phase open suspends for a while: 2^18 polls are about a second.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
+    for (uint32_t i = 0; i < (1u << 18); ++i)
+        if (tc::mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+// The same for a whole warp, which stays together whatever its lanes saw.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)); }
+// The A operand from tensor memory: lane = row, one 32-bit column = two consecutive fp16 elements along K.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+// fp32 accumulator, fp16 A and B, A K-major, B K-major or MN-major
+__host__ __device__ constexpr uint32_t idesc(uint32_t M, uint32_t N, uint32_t b_mn_major) {
+    return tc::idesc_f16_kmajor(M, N) | (b_mn_major << 16);
+}
+__device__ __forceinline__ TreePiece load_piece(const TreePiece* p) {
+    TreePiece out;
+    const uint4* src = reinterpret_cast<const uint4*>(p);
+    uint4* dst = reinterpret_cast<uint4*>(&out);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) dst[i] = __ldg(src + i);
+    return out;
+}
+// Bit 15 / 31 of the result: the lower / upper fp16 of w is infinite or NaN.
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+
+// Puts query row `row` (or zeros) into the swizzled operand tile(s); returns what the scores have to be multiplied with
+// to undo the row's scaling.
+template <int D, bool EXACT>
+__device__ __forceinline__ float load_query_row(uint32_t sQ, uint32_t row, const void* q, int q_f32, bool valid, size_t elem) {
+    const uint32_t base = sQ + (row >> 3) * 1024u + (row & 7u) * 128u;
+    auto at = [&](uint32_t c) { return base + (c >> 3) * kSlabQ + (((c ^ row) & 7u) << 4); };
+    if constexpr (!EXACT) {
+        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(q) + elem);
+#pragma unroll
+        for (uint32_t c = 0; c < D / 8; ++c) st_shared16(at(c), valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0));
+        return 1.0f;
+    } else {
+        auto load8 = [&](uint32_t c, float (&x)[8]) {
+            if (q_f32) {
+                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + elem) + 2 * c;
+                const float4 a = __ldg(src), b = __ldg(src + 1);
+                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+            } else {
+                const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(q) + elem) + c);
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+                    x[2 * i] = f.x; x[2 * i + 1] = f.y;
+                }
+            }
+        };
+        float top = 0.f;
+        if (valid) {
+#pragma unroll 4
+            for (uint32_t c = 0; c < D / 8; ++c) {
+                float x[8];
+                load8(c, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+            }
+        }
+        // largest magnitude to [2^7, 2^8): well inside fp16, and the low halves stay clear of its subnormals
+        int shift = 0;
+        if (top > 0.f && top < INFINITY) shift = max(-120, min(120, 7 - ilogbf(top)));
+        const float up = __int_as_float((127 + shift) << 23), down = __int_as_float((127 - shift) << 23);
+#pragma unroll 4
+        for (uint32_t c = 0; c < D / 8; ++c) {
+            float x[8] = {};
+            if (valid) load8(c, x);
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+                const __half2 h = __floats2half2_rn(a, b);
+                const float2 back = __half22float2(h);
+                hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                lo[i] = pack(a - back.x, b - back.y);
+            }
+            st_shared16(at(c), make_uint4(hi[0], hi[1], hi[2], hi[3]));
+            st_shared16(at(c) + (D / 64) * kSlabQ, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        }
+        return down;
+    }
+}
+
+template <int D, bool EXACT>
+__global__ void __launch_bounds__(kThreads, (Config<D, EXACT>::ctas))
+paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                          const __grid_constant__ TreeParams prm) {
+    using C = Config<D, EXACT>;
+    constexpr uint32_t STAGES = C::stages;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    Bars<STAGES>& bars = *reinterpret_cast<Bars<STAGES>*>(smem_raw + C::tile_bytes);
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t base = smem_u32(smem_raw);
+    if (base & 1023u) {   // the swizzle needs it; never expected
+        if (threadIdx.x == 0) atomicOr(prm.err, MLC_DEVERR_WAIT_TIMEOUT | (0x50u << 8));
+        return;
+    }
+    const uint32_t sQ = base, sKV = base + C::q_bytes;   // stage s: K at sKV + s * 2 * kv_bytes, V right behind it
+    if (threadIdx.x == 0) {
+        tc::mbar_init(smem_u32(&bars.q_full), 128);
+        for (uint32_t s = 0; s < STAGES; ++s) {
+            tc::mbar_init(smem_u32(&bars.k_full[s]), 1);
+            tc::mbar_init(smem_u32(&bars.k_empty[s]), 1);
+            tc::mbar_init(smem_u32(&bars.v_full[s]), 1);
+            tc::mbar_init(smem_u32(&bars.v_empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            tc::mbar_init(smem_u32(&bars.s_full[b]), 1);
+            tc::mbar_init(smem_u32(&bars.p_full[b]), 128);   // two, like the S buffers: softmax may be a tile ahead of the MMA warp
+        }
+        tc::mbar_init(smem_u32(&bars.pv_done), 1);
+        bars.not_finite = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 4) tc::tmem_alloc(smem_u32(&bars.tmem_slot), kTmemCols);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = bars.tmem_slot;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    const uint32_t first = __ldg(prm.cta_off + blockIdx.x), last = __ldg(prm.cta_off + blockIdx.x + 1);
+    // A wait that ran out: which wait (bits 8-15 of the error word) and at which tile (bits 16-31).
+    auto give_up = [&](uint32_t where, uint32_t tile) {
+        if (lane == 0 && atomicCAS(prm.err, 0u, MLC_DEVERR_WAIT_TIMEOUT | (where << 8) | (tile << 16)) != 0u)
+            atomicOr(prm.err, MLC_DEVERR_WAIT_TIMEOUT);
+    };
+
+    if (warp >= 5) {
+        // ---------------- TMA producers: warp 5 the K tiles, warp 6 the V tiles ----------------
+        // Each has its own ring: a K tile is free when its Q.K^T is done, a V tile only after its P.V.
+        const bool is_v = warp == 6;
+        const CUtensorMap* map = is_v ? &tmV : &tmK;
+        uint64_t* full = is_v ? bars.v_full : bars.k_full;
+        uint64_t* empty = is_v ? bars.v_empty : bars.k_empty;
+        const uint32_t ring = sKV + (is_v ? C::kv_bytes : 0u);
+        uint32_t g = 0;   // tiles of this CTA so far
+        bool ok = true;
+        for (uint32_t pi = first; ok && pi < last; ++pi) {
+            const TreePiece p = load_piece(prm.pieces + pi);
+            const uint32_t len = p.prefix + p.draft;
+            const uint32_t token_begin = p.tile_begin * kTreeTile;
+            // boxes of the piece that hold tokens; their page ids are fetched 32 at a time, a lane each
+            const uint32_t n_boxes = (min(len, token_begin + p.n_tiles * kTreeTile) - token_begin + prm.box_rows - 1) / prm.box_rows;
+            uint32_t box = 0, ids = 0;
+            for (uint32_t j = 0; j < p.n_tiles; ++j, ++g) {
+                const uint32_t s = g % STAGES;
+                if (g >= STAGES && !warp_wait(smem_u32(&empty[s]), (g / STAGES - 1) & 1u)) {
+                    give_up(is_v ? 0x31 : 0x30, g);
+                    ok = false;
+                    break;
+                }
+                const uint32_t in_tile = min(prm.boxes, n_boxes - box);
+                const uint32_t bar = smem_u32(&full[s]), dst = ring + s * 2 * C::kv_bytes;
+                if (lane == 0) expect_tx(bar, in_tile * prm.box_rows * D * 2);
+                for (uint32_t b = 0; b < in_tile; ++b, ++box) {
+                    if ((box & 31u) == 0) {
+                        const uint32_t mine = box + lane;
+                        ids = mine < n_boxes ? __ldg(prm.pt_flat + p.pt_off + (token_begin + mine * prm.box_rows) / prm.P) : 0u;
+                    }
+                    const int page = static_cast<int>(__shfl_sync(0xffffffffu, ids, box & 31u));
+                    const int slot = static_cast<int>((token_begin + box * prm.box_rows) % prm.P);
+                    if (lane == 0) {
+#pragma unroll
+                        for (uint32_t c = 0; c < C::slabs; ++c)
+                            tma_load_4d(dst + c * kSlabKV + b * prm.box_rows * 128, map, bar, static_cast<int>(c * 64),
+                                        static_cast<int>(p.kv_head), slot, page);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok && lane == 0) {   // copies in flight must land before the CTA ends
+            for (uint32_t t = g > STAGES ? g - STAGES : 0; t < g; ++t) wait(smem_u32(&full[t % STAGES]), (t / STAGES) & 1u);
+        }
+    } else if (warp == 4) {
+        // ---------------- MMA issue: the warp walks the loop together, one elected lane issues ----------------
+        constexpr uint32_t idesc_qk = idesc(kTreeRows, kTreeTile, 0);   // B = K tile, K-major
+        constexpr uint32_t idesc_pv = idesc(kTreeRows, D, 1);           // B = V tile, MN-major
+        const uint64_t desc_k = tc::smem_desc_sw128(0, 16, 1024);
+        const uint64_t desc_v = tc::smem_desc_sw128(0, kSlabKV, 1024);
+        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0), sQ_u = __shfl_sync(0xffffffffu, sQ, 0);
+        const uint32_t sKV_u = sQ_u + C::q_bytes;
+        auto issue_qk = [&](uint32_t g) {
+            const uint32_t s = g % STAGES, sK = sKV_u + s * 2 * C::kv_bytes, d = tmem_u + kTmemS + (g & 1u) * kTreeTile;
+            if (tc::elect_one()) {
+#pragma unroll
+                for (uint32_t half = 0; half < (EXACT ? 2u : 1u); ++half)
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 16; ++k) {
+                        const uint32_t a = sQ_u + (half * C::slabs + (k >> 2)) * kSlabQ + (k & 3) * 32;
+                        const uint32_t b = sK + (k >> 2) * kSlabKV + (k & 3) * 32;
+                        tc::mma_f16(d, desc_k | (a >> 4), desc_k | (b >> 4), idesc_qk, half + k > 0);
+                    }
+                tc::commit(smem_u32(&bars.k_empty[s]));
+                tc::commit(smem_u32(&bars.s_full[g & 1u]));
+            }
+            __syncwarp();
+        };
+        uint32_t g = 0, where = 0x10, issued_qk = 0, issued_pv = 0;
+        bool ok = true;
+        auto all_wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) {
+            where = code;
+            return warp_wait(smem_u32(bar), parity);
+        };
+        // Q.K^T of tile t: its K has landed, and P of tile t - 2, which lies in the same buffer, has been used. The wait is
+        // for the newest P.V issued (t - 2 inside a piece, t - 1 at its start): a parity wait for an older phase would be ambiguous.
+        auto start_tile = [&](uint32_t t) {
+            if (!all_wait(&bars.k_full[t % STAGES], (t / STAGES) & 1u, 0x11)) return false;
+            if (issued_pv && !all_wait(&bars.pv_done, (issued_pv - 1) & 1u, 0x12)) return false;
+            tc::fence_after();
+            issue_qk(t);
+            issued_qk = t + 1;
+            return true;
+        };
+        for (uint32_t pi = first; ok && pi < last; ++pi) {
+            const uint32_t n_tiles = __ldg(&prm.pieces[pi].n_tiles);
+            if (!all_wait(&bars.q_full, (pi - first) & 1u, 0x10) || !start_tile(g)) {
+                ok = false;
+                break;
+            }
+            for (uint32_t j = 0; j < n_tiles; ++j, ++g) {
+                if (j + 1 < n_tiles && !start_tile(g + 1)) { ok = false; break; }   // runs under this tile's softmax
+                const uint32_t s = g % STAGES;
+                if (!all_wait(&bars.v_full[s], (g / STAGES) & 1u, 0x13) || !all_wait(&bars.p_full[g & 1u], (g >> 1) & 1u, 0x14)) {
+                    ok = false;
+                    break;
+                }
+                tc::fence_after();
+                const uint32_t sV = sKV_u + s * 2 * C::kv_bytes + C::kv_bytes;
+                const uint32_t P = tmem_u + kTmemS + (g & 1u) * kTreeTile;
+                if (tc::elect_one()) {
+#pragma unroll
+                    for (uint32_t half = 0; half < (EXACT ? 2u : 1u); ++half)
+#pragma unroll
+                        for (uint32_t k = 0; k < kTreeTile / 16; ++k)   // 16 tokens per step: 8 columns of P, 16 rows of V
+                            mma_f16_ts(tmem_u, P + half * 32 + k * 8, desc_v | ((sV + k * 16 * 128) >> 4), idesc_pv,
+                                       j > 0 || half + k > 0);
+                    tc::commit(smem_u32(&bars.v_empty[s]));
+                    tc::commit(smem_u32(&bars.pv_done));
+                }
+                __syncwarp();
+                issued_pv = g + 1;
+            }
+        }
+        if (!ok) {   // nothing may still read shared or tensor memory when the CTA ends
+            give_up(where, g);
+            if (issued_qk) wait(smem_u32(&bars.s_full[(issued_qk - 1) & 1u]), ((issued_qk - 1) >> 1) & 1u);
+            if (issued_pv) wait(smem_u32(&bars.pv_done), (issued_pv - 1) & 1u);
+        }
+    } else {
+        // ---------------- softmax and output: thread = query row ----------------
+        const uint32_t row = threadIdx.x, lane_base = (warp * 32u) << 16;
+        uint32_t g = 0, where = 0x20;
+        bool ok = true;
+        float row_down = 1.0f;
+        TreePiece p = load_piece(prm.pieces + first);
+        auto put_query = [&](const TreePiece& pc) {
+            const uint32_t r = pc.row_begin + row;
+            const size_t elem = (static_cast<size_t>(pc.token0 + r / prm.G) * prm.H + pc.kv_head * prm.G + r % prm.G) * D;
+            row_down = load_query_row<D, EXACT>(sQ, row, prm.q, prm.q_f32, row < pc.n_rows, elem);
+            tc::fence_proxy_async_smem();
+            tc::mbar_arrive(smem_u32(&bars.q_full));
+        };
+        if (first < last) put_query(p);
+        for (uint32_t pi = first; ok && pi < last; ++pi) {
+            const uint32_t len = p.prefix + p.draft;
+            const bool busy = warp * 32u < p.n_rows;   // the warp has rows
+            const uint32_t r = p.row_begin + min(row, p.n_rows - 1);
+            const uint32_t* mask = prm.mask + static_cast<size_t>(p.token0 + r / prm.G) * prm.mask_words;
+            const float scale = prm.scale_log2 * row_down;      // of a raw score, base-2 units
+            const float rescale_step = 8.0f / scale;
+            float m_ref = -INFINITY, l_sum = 0.f;               // reference maximum (raw scores) of the accumulator, row sum
+            for (uint32_t j = 0; j < p.n_tiles; ++j, ++g) {
+                const uint32_t kv0 = (p.tile_begin + j) * kTreeTile;
+                where = 0x20;
+                ok = warp_wait(smem_u32(&bars.s_full[g & 1u]), (g >> 1) & 1u);
+                if (!ok) break;
+                tc::fence_after();
+                if (busy) {
+                    uint32_t s[64];
+                    {
+                        uint32_t lo[32], hi[32];
+                        tc::tmem_ld32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile, lo);
+                        tc::tmem_ld32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile + 32, hi);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) { s[i] = lo[i]; s[32 + i] = hi[i]; }
+                    }
+                    if (kv0 + kTreeTile > p.prefix) {
+                        // 64 bits of what the row sees: committed tokens, then its mask from drafted token j0 on
+                        const uint32_t committed = p.prefix > kv0 ? p.prefix - kv0 : 0u;
+                        const uint32_t j0 = kv0 > p.prefix ? kv0 - p.prefix : 0u;
+                        const uint32_t w = j0 >> 5, sh = j0 & 31u;
+                        auto word = [&](uint32_t i) { return i < prm.mask_words ? __ldg(mask + i) : 0u; };
+                        const uint32_t w0 = word(w), w1 = word(w + 1), w2 = word(w + 2);
+                        uint64_t see = static_cast<uint64_t>(__funnelshift_r(w0, w1, sh)) |
+                                       (static_cast<uint64_t>(__funnelshift_r(w1, w2, sh)) << 32);
+                        if (committed) see = (see << committed) | ((uint64_t(1) << committed) - 1);
+                        if (len - kv0 < kTreeTile) see &= (uint64_t(1) << (len - kv0)) - 1;
+                        const uint32_t see_lo = static_cast<uint32_t>(see), see_hi = static_cast<uint32_t>(see >> 32);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            if (!((see_lo >> c) & 1u)) s[c] = 0xff800000u;        // -inf
+                            if (!((see_hi >> c) & 1u)) s[32 + c] = 0xff800000u;
+                        }
+                    }
+                    float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 64; c += 4) {
+                        t0 = fmaxf(t0, __uint_as_float(s[c]));
+                        t1 = fmaxf(t1, __uint_as_float(s[c + 1]));
+                        t2 = fmaxf(t2, __uint_as_float(s[c + 2]));
+                        t3 = fmaxf(t3, __uint_as_float(s[c + 3]));
+                    }
+                    const float m_new = fmaxf(m_ref, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
+                    const bool need = m_new > m_ref + rescale_step || (m_ref == -INFINITY && m_new > -INFINITY);
+                    const float alpha = need ? (m_ref == -INFINITY ? 0.f : ex2((m_ref - m_new) * scale)) : 1.0f;
+                    if (need) m_ref = m_new;
+                    l_sum *= alpha;
+                    const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref * scale;
+                    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t hi[32], lo[EXACT ? 32 : 1];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), scale, neg_m));
+                        const float p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale, neg_m));
+                        ps[i & 3] += p0 + p1;
+                        const __half2 h = __floats2half2_rn(p0, p1);
+                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        if constexpr (EXACT) {
+                            const float2 back = __half22float2(h);
+                            lo[i] = pack(p0 - back.x, p1 - back.y);
+                        }
+                    }
+                    l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+                    if (j > 0 && __any_sync(0xffffffffu, need)) {
+                        where = 0x21;
+                        ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
+                        if (!ok) break;
+                        tc::fence_after();
+#pragma unroll 1
+                        for (int c0 = 0; c0 < D; c0 += 32) {
+                            uint32_t o[32];
+                            tc::tmem_ld32(tmem + lane_base + c0, o);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_st32(tmem + lane_base + c0, o);
+                        }
+                        tmem_wait_st();
+                    }
+                    // P over this tile's scores (own lane, already read): the halves in 32 columns each
+                    tmem_st32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile, hi);
+                    if constexpr (EXACT) tmem_st32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile + 32, lo);
+                    tmem_wait_st();
+                }
+                if (kv0 + kTreeTile > p.prefix) {
+                    // V rows of drafted tokens lose what is not finite, rows behind the last token become zeros
+                    const uint32_t s = g % STAGES;
+                    where = 0x22;
+                    ok = warp_wait(smem_u32(&bars.v_full[s]), (g / STAGES) & 1u);
+                    if (!ok) break;
+                    const uint32_t from = p.prefix > kv0 ? p.prefix - kv0 : 0u, end = min(len - kv0, kTreeTile);
+                    const uint32_t sV = sKV + s * 2 * C::kv_bytes + C::kv_bytes;
+                    for (uint32_t i = row; i < (kTreeTile - from) * (D / 8); i += 128) {
+                        const uint32_t vr = from + i / (D / 8), c = i % (D / 8);
+                        const uint32_t addr = sV + (c >> 3) * kSlabKV + vr * 128 + ((c & 7) << 4);
+                        if (vr >= end) {
+                            st_shared16(addr, make_uint4(0, 0, 0, 0));
+                            continue;
+                        }
+                        uint4 x = ld_shared16(addr);
+                        uint32_t* w = &x.x;
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t bad = not_finite(w[k]);
+                            w[k] &= ~((bad >> 15) * 0xFFFFu);
+                            any |= bad;
+                        }
+                        if (any) {
+                            st_shared16(addr, x);
+                            *reinterpret_cast<volatile uint32_t*>(&bars.not_finite) = pi + 1;
+                        }
+                    }
+                    tc::fence_proxy_async_smem();
+                }
+                // Every warp follows pv_done phase by phase (a parity wait is only unambiguous for a waiter at most
+                // one phase behind). It costs nothing: P.V of this tile cannot start before the one before is done.
+                if (g > 0) {
+                    where = 0x24;
+                    ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
+                    if (!ok) break;
+                }
+                tc::fence_before();
+                tc::mbar_arrive(smem_u32(&bars.p_full[g & 1u]));
+            }
+            if (!ok) break;
+            // every Q.K^T of this piece is done: the next one's queries may move in while the last P.V runs
+            const TreePiece done = p;
+            if (pi + 1 < last) {
+                p = load_piece(prm.pieces + pi + 1);
+                put_query(p);
+            }
+            where = 0x23;
+            ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
+            if (!ok) break;
+            tc::fence_after();
+            if (busy) {
+                const bool mine = row < done.n_rows;
+                const bool whole = done.slot == kTreeNoSlot;
+                const float inv = whole ? (l_sum == 0.f ? 0.f : 1.0f / l_sum) : 1.0f;
+                const size_t out = (static_cast<size_t>(done.token0 + r / prm.G) * prm.H + done.kv_head * prm.G + r % prm.G) * D;
+                const size_t part = static_cast<size_t>(done.slot) * prm.slot_rows + row;
+                const bool repair = *reinterpret_cast<volatile uint32_t*>(&bars.not_finite) == pi + 1;
+                if (!whole && mine) prm.part_ml[part] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * scale, l_sum);
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t o[32];
+                    tc::tmem_ld32(tmem + lane_base + c0, o);
+                    tc::tmem_wait_ld();
+                    if (!mine) continue;
+                    if (repair) {
+                        // drafted tokens of this piece that the row sees: what is not finite in V belongs in its output
+                        const uint32_t begin = done.tile_begin * kTreeTile, stop = min(len, begin + done.n_tiles * kTreeTile);
+                        for (uint32_t pos = max(begin, done.prefix); pos < stop; ++pos) {
+                            const uint32_t t = pos - done.prefix;
+                            if (!((__ldg(mask + (t >> 5)) >> (t & 31u)) & 1u)) continue;
+                            const size_t page = __ldg(prm.pt_flat + done.pt_off + pos / prm.P);
+                            const __half* v = prm.v_pages + ((page * prm.P + pos % prm.P) * prm.KVH + done.kv_head) * D + c0;
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float x = __half2float(v[i]);
+                                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
+                            }
+                        }
+                    }
+                    if (!whole) {
+                        float4* dst = reinterpret_cast<float4*>(prm.part_o + part * D + c0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
+                                                 __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    } else if (prm.o_f32) {
+                        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(prm.o) + out + c0);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
+                                                 __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
+                    } else {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(prm.o) + out + c0);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            dst[i] = make_uint4(pack(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
+                                                pack(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
+                                                pack(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
+                                                pack(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
+                    }
+                }
+            }
+        }
+        if (!ok) give_up(where, g);
+    }
+    // every tcgen05 operation is finished: free the tensor memory
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 4) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+// O of the rows whose unit was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. WARPS warps per row
+// take the parts round-robin; a lane holds D / 32 columns.
+template <int D, int WARPS, typename OT>
+__global__ void __launch_bounds__(128) tree_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
+                                                         const TreeSplit* __restrict__ splits, const uint32_t* __restrict__ row_split,
+                                                         OT* __restrict__ o, uint32_t rows, uint32_t slot_rows, uint32_t H, uint32_t G) {
+    constexpr int V = D / 32;
+    constexpr int kRowsPerCta = 4 / WARPS;
+    __shared__ float s_o[WARPS > 1 ? WARPS : 1][D];
+    __shared__ float2 s_ml[4];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t row = blockIdx.x * kRowsPerCta + warp / WARPS, sub = warp % WARPS;
+    if (row >= rows) return;   // with WARPS > 1 a CTA has one row: all or none leave
+    const TreeSplit sp = splits[row_split[row]];
+    const uint32_t r = row - sp.first_row;
+    auto index = [&](uint32_t k) { return static_cast<size_t>(sp.first_slot + k) * slot_rows + r; };
+    float top = -INFINITY;
+    for (uint32_t k = sub * 32 + lane; k < sp.n_parts; k += WARPS * 32) top = fmaxf(top, __ldcg(&part_ml[index(k)]).x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if constexpr (WARPS > 1) {
+        if (lane == 0) s_ml[warp].x = top;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_ml[w].x);
+        __syncthreads();
+    }
+    float acc[V] = {}, l = 0.f;
+#pragma unroll 4
+    for (uint32_t k = sub; k < sp.n_parts; k += WARPS) {
+        const float2 ml = __ldcg(&part_ml[index(k)]);
+        const float* src = part_o + index(k) * D + lane * V;
+        float v[V];
+        if constexpr (V == 4) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
+            v[0] = x.x; v[1] = x.y;
+        }
+        // a part that saw nothing has m = -inf, l = 0 and o = 0
+        const float w = ml.x == -INFINITY ? 1.0f : ex2(ml.x - top);
+        l += ml.y * w;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += v[i] * w;
+    }
+    if constexpr (WARPS > 1) {
+        if (lane == 0) s_ml[warp].y = l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) s_o[sub][lane * V + i] = acc[i];
+        __syncthreads();
+        if (sub) return;
+        l = 0.f;
+        for (int w = 0; w < WARPS; ++w) l += s_ml[w].y;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            acc[i] = 0.f;
+            for (int w = 0; w < WARPS; ++w) acc[i] += s_o[w][lane * V + i];
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const uint32_t rr = sp.row_begin + r;
+    OT* dst = o + (static_cast<size_t>(sp.token0 + rr / G) * H + sp.kv_head * G + rr % G) * D + lane * V;
+    if constexpr (sizeof(OT) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) dst[i] = acc[i] * inv;
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack(acc[i] * inv, acc[i + 1] * inv);
+    }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int pool_map(mlc_ctx* ctx, CUtensorMap* out, const void* pool, const TreeShape& s, uint32_t box_rows) {
+    if (!ctx->tmap_encode_fn) {
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ctx->tmap_encode_fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess || !ctx->tmap_encode_fn)
+            return ctx->fail(MLC_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    }
+    const cuuint64_t dims[4] = {s.D, s.KVH, s.P, s.capacity};
+    const cuuint64_t strides[3] = {s.D * 2, s.KVH * s.D * 2, s.P * s.KVH * s.D * 2};
+    const cuuint32_t box[4] = {64, 1, box_rows, 1}, unit[4] = {1, 1, 1, 1};
+    const CUresult r = reinterpret_cast<EncodeTiledFn>(ctx->tmap_encode_fn)(
+        out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(pool), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return ctx->fail(MLC_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+    return MLC_OK;
+}
+
+template <int D, typename OT>
+cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const float* part_o, const float2* part_ml, void* o) {
+    // few rows: four warps share one, the parts are read four at a time
+    const bool wide = v.merge_rows <= 4u * static_cast<uint32_t>(ctx->sm_count) * 4u;
+    auto kernel = wide ? tree_merge_kernel<D, 4, OT> : tree_merge_kernel<D, 1, OT>;
+    const dim3 grid(wide ? v.merge_rows : (v.merge_rows + 3) / 4);
+    return launch_dependent(ctx, kernel, grid, 128, 0, part_o, part_ml, v.splits, v.row_split, static_cast<OT*>(o), v.merge_rows,
+                            v.slot_rows, static_cast<uint32_t>(s.H), static_cast<uint32_t>(s.H / s.KVH));
+}
+
+template <int D, bool EXACT>
+int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a) {
+    using C = Config<D, EXACT>;
+    constexpr size_t smem = C::tile_bytes + sizeof(Bars<C::stages>);
+    const uint32_t box_rows = static_cast<uint32_t>(s.P < kTreeTile ? s.P : kTreeTile);
+    CUtensorMap mk, mv;
+    int st = pool_map(ctx, &mk, a.k_pages, s, box_rows);
+    if (st == MLC_OK) st = pool_map(ctx, &mv, a.v_pages, s, box_rows);
+    if (st != MLC_OK) return st;
+    bool& opted = ctx->tree_smem_set[(D == 128 ? 2 : 0) + (EXACT ? 1 : 0)];
+    if (!opted) {
+        MLCB_CUDA(ctx, cudaFuncSetAttribute(paged_tree_tcgen05_kernel<D, EXACT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                            static_cast<int>(smem)));
+        opted = true;
+    }
+    TreeParams p{};
+    p.q = a.q;
+    p.v_pages = static_cast<const __half*>(a.v_pages);
+    p.o = a.o;
+    if (v.n_slots) {
+        p.part_o = static_cast<float*>(ctx->tree_scratch.dev);
+        p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(v.n_slots) * v.slot_rows * D);
+    }
+    p.pieces = v.pieces;
+    p.cta_off = v.cta_off;
+    p.pt_flat = v.pt_flat;
+    p.mask = v.mask;
+    p.err = ctx->d_err;
+    p.H = static_cast<uint32_t>(s.H);
+    p.KVH = static_cast<uint32_t>(s.KVH);
+    p.G = static_cast<uint32_t>(s.H / s.KVH);
+    p.P = static_cast<uint32_t>(s.P);
+    p.mask_words = static_cast<uint32_t>(s.mask_words);
+    p.slot_rows = v.slot_rows;
+    p.box_rows = box_rows;
+    p.boxes = kTreeTile / box_rows;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.q_f32 = a.q_dtype == MLC_F32;
+    p.o_f32 = a.o_dtype == MLC_F32;
+    MLCB_CUDA(ctx, launch_dependent(ctx, paged_tree_tcgen05_kernel<D, EXACT>, dim3(v.n_cta), kThreads, smem, mk, mv, p));
+    ++ctx->launches;
+    if (!v.n_slots) return MLC_OK;
+    if (a.o_dtype == MLC_F32) MLCB_CUDA(ctx, (merge_launch<D, float>(ctx, s, v, p.part_o, p.part_ml, a.o)));
+    else MLCB_CUDA(ctx, (merge_launch<D, __half>(ctx, s, v, p.part_o, p.part_ml, a.o)));
+    ++ctx->launches;
+    return MLC_OK;
+}
+
+}  // namespace
+
+bool tree_tcgen05_shape(const TreeShape& s) {
+    const bool pages = s.P % kTreeTile == 0 || s.P == 32 || s.P == 16;
+    return (s.D == 64 || s.D == 128) && pages && s.capacity > 0 && s.capacity < (size_t(1) << 31) && s.P < (size_t(1) << 31) &&
+           s.KVH < (size_t(1) << 31) && s.P * s.KVH * s.D * 2 < (size_t(1) << 40);
+}
+
+bool tree_tcgen05_buffers(const TreeArgs& a) {
+    return aligned_to(a.q, 16) && aligned_to(a.o, 16) && aligned_to(a.k_pages, 16) && aligned_to(a.v_pages, 16);
+}
+
+size_t tree_scratch_bytes(const TreeShape& s, uint32_t n_slots, uint32_t slot_rows) {
+    return static_cast<size_t>(n_slots) * slot_rows * (s.D * sizeof(float) + sizeof(float2));
+}
+
+int launch_tree_tcgen05(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a) {
+    const bool exact = a.q_dtype == MLC_F32 || a.o_dtype == MLC_F32;
+    if (s.D == 64) return exact ? launch_t<64, true>(ctx, s, v, a) : launch_t<64, false>(ctx, s, v, a);
+    return exact ? launch_t<128, true>(ctx, s, v, a) : launch_t<128, false>(ctx, s, v, a);
+}
+
+}  // namespace mlcb

@@ -69,7 +69,7 @@ struct mlc_ctx {
     int sm_count = 0;
     int force_general = 0;
     uint32_t wait_limit = 0;        // polls before a flag wait gives up; 0 = the kernel's default (about a second)
-    int last_attention_kernel = 0;  // 0 none yet, 1 general, 2 TMA / tensor-core
+    int last_attention_kernel = 0;  // 0 none yet, 1 general, 2 TMA / tensor-core, 3 prefill, 4 tree
     uint64_t launches = 0;
     uint64_t sync_epoch = 1;        // counts full synchronisations of the stream (mlc_pass_flush): work enqueued in an earlier epoch is done
     uint64_t allocations = 0;       // device and pinned-host allocations made through this context
@@ -90,6 +90,7 @@ struct mlc_ctx {
     uint32_t* d_counters = nullptr;
     size_t n_counters = 0;
     size_t decode_smem_set[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};  // dynamic-smem opt-in already applied, per kernel variant
+    bool tree_smem_set[4] = {false, false, false, false};   // same, for the variants of the tree attention kernel
     bool prefill_smem_set = false;             // same, for the chunked-prefill kernel
     // copy streams and events of the host-buffer decode pass (created on first use)
     cudaStream_t h2d_stream = nullptr, d2h_stream = nullptr;

@@ -32,15 +32,15 @@ static constexpr uint32_t kTreeNoSlot = 0xFFFFFFFFu;
 struct TreePiece {
     uint32_t kv_head, row_begin, n_rows;   // rows of the unit, row = drafted token * group + head of the group
     uint32_t tile_begin, n_tiles;
-    uint32_t slot;                         // where the partial goes; kTreeNoSlot: the piece is the whole unit
+    uint32_t slot;                         // where the partial goes; kTreeNoSlot: the piece is the whole run
     uint32_t prefix, draft, token0, pt_off;
     uint32_t pad[2];
 };
 static_assert(sizeof(TreePiece) == 48, "read as three 16-byte vectors");
 
-// A unit that was cut: its partials lie in n_parts consecutive slots.
+// A row tile whose run was cut: part k lies in slot first_slot + k * slot_step.
 struct TreeSplit {
-    uint32_t kv_head, row_begin, n_rows, token0, first_slot, n_parts, first_row, pad;
+    uint32_t kv_head, row_begin, n_rows, token0, first_slot, n_parts, first_row, slot_step;
 };
 static_assert(sizeof(TreeSplit) == 32, "read as two 16-byte vectors");
 

@@ -40,6 +40,7 @@ constexpr uint32_t kSlabKV = kTreeTile * 128;  // 64 halfs of every token of a t
 constexpr uint32_t kTmemCols = 256;            // O: up to 128 columns, S: 2 x 64
 constexpr uint32_t kTmemS = 128;
 constexpr uint32_t kThreads = 224;
+constexpr int kFmaPairs = 12;                  // of a tile's 32 pairs of columns: exponentials on the FMA pipe
 
 template <int D, bool EXACT>
 struct Config {
@@ -79,6 +80,40 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// NaN if one of the three is.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// Two fp32 operations in one instruction, on register pairs.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)),
+        "l"(*reinterpret_cast<uint64_t*>(&c)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+// 2^x for two x <= 127 on the FMA pipe: 2^n times a cubic for 2^f, n = rint(x), f = x - n in [-1/2, 1/2]. The coefficients are
+// the minimax ones for the relative error, 2^-13.7 (least squares reweighted until the error is level). x below -126 gives less
+// than 2^-125.
+__device__ __forceinline__ float2 ex2_fma(float2 x) {
+    const float magic = 12582912.0f;   // 1.5 * 2^23: adding it leaves rint(x) in the low bits
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const float2 t = add2(x, make_float2(magic, magic));
+    const float2 n = add2(t, make_float2(-magic, -magic));
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
+    p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
+    p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
+    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
+                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -400,81 +435,96 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 if (!ok) break;
                 tc::fence_after();
                 if (busy) {
-                    uint32_t s[64];
-                    {
-                        uint32_t lo[32], hi[32];
-                        tc::tmem_ld32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile, lo);
-                        tc::tmem_ld32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile + 32, hi);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) { s[i] = lo[i]; s[32 + i] = hi[i]; }
-                    }
-                    if (kv0 + kTreeTile > p.prefix) {
-                        // 64 bits of what the row sees: committed tokens, then its mask from drafted token j0 on
-                        const uint32_t committed = p.prefix > kv0 ? p.prefix - kv0 : 0u;
-                        const uint32_t j0 = kv0 > p.prefix ? kv0 - p.prefix : 0u;
-                        const uint32_t w = j0 >> 5, sh = j0 & 31u;
-                        auto word = [&](uint32_t i) { return i < prm.mask_words ? __ldg(mask + i) : 0u; };
-                        const uint32_t w0 = word(w), w1 = word(w + 1), w2 = word(w + 2);
-                        uint64_t see = static_cast<uint64_t>(__funnelshift_r(w0, w1, sh)) |
-                                       (static_cast<uint64_t>(__funnelshift_r(w1, w2, sh)) << 32);
-                        if (committed) see = (see << committed) | ((uint64_t(1) << committed) - 1);
-                        if (len - kv0 < kTreeTile) see &= (uint64_t(1) << (len - kv0)) - 1;
-                        const uint32_t see_lo = static_cast<uint32_t>(see), see_hi = static_cast<uint32_t>(see >> 32);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            if (!((see_lo >> c) & 1u)) s[c] = 0xff800000u;        // -inf
-                            if (!((see_hi >> c) & 1u)) s[32 + c] = 0xff800000u;
-                        }
-                    }
-                    float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 64; c += 4) {
-                        t0 = fmaxf(t0, __uint_as_float(s[c]));
-                        t1 = fmaxf(t1, __uint_as_float(s[c + 1]));
-                        t2 = fmaxf(t2, __uint_as_float(s[c + 2]));
-                        t3 = fmaxf(t3, __uint_as_float(s[c + 3]));
-                    }
-                    const float m_new = fmaxf(m_ref, fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)));
-                    const bool need = m_new > m_ref + rescale_step || (m_ref == -INFINITY && m_new > -INFINITY);
-                    const float alpha = need ? (m_ref == -INFINITY ? 0.f : ex2((m_ref - m_new) * scale)) : 1.0f;
-                    if (need) m_ref = m_new;
-                    l_sum *= alpha;
-                    const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref * scale;
-                    float ps[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint32_t tS = tmem + lane_base + kTmemS + (g & 1u) * kTreeTile;
                     uint32_t hi[32], lo[EXACT ? 32 : 1];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float p0 = ex2(fmaf(__uint_as_float(s[2 * i]), scale, neg_m));
-                        const float p1 = ex2(fmaf(__uint_as_float(s[2 * i + 1]), scale, neg_m));
-                        ps[i & 3] += p0 + p1;
-                        const __half2 h = __floats2half2_rn(p0, p1);
-                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                        if constexpr (EXACT) {
-                            const float2 back = __half22float2(h);
-                            lo[i] = pack(p0 - back.x, p1 - back.y);
-                        }
-                    }
-                    l_sum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-                    if (j > 0 && __any_sync(0xffffffffu, need)) {
-                        where = 0x21;
-                        ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
-                        if (!ok) break;
-                        tc::fence_after();
-#pragma unroll 1
-                        for (int c0 = 0; c0 < D; c0 += 32) {
-                            uint32_t o[32];
-                            tc::tmem_ld32(tmem + lane_base + c0, o);
+                    // First with the reference maximum as it is: the exponentials need not wait for the tile's maximum, which
+                    // is found beside them. Where some row's maximum has outgrown its reference (or is NaN), and on a run's
+                    // first tile, the tile is done (again) with a new reference.
+                    for (bool moved = j == 0;; moved = true) {
+                        uint32_t s[64];
+                        {
+                            uint32_t a[32], b[32];
+                            tc::tmem_ld32(tS, a);
+                            tc::tmem_ld32(tS + 32, b);
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                            tmem_st32(tmem + lane_base + c0, o);
+                            for (int i = 0; i < 32; ++i) { s[i] = a[i]; s[32 + i] = b[i]; }
                         }
-                        tmem_wait_st();
+                        if (kv0 + kTreeTile > p.prefix) {
+                            // 64 bits of what the row sees: committed tokens, then its mask from drafted token j0 on
+                            const uint32_t committed = p.prefix > kv0 ? p.prefix - kv0 : 0u;
+                            const uint32_t j0 = kv0 > p.prefix ? kv0 - p.prefix : 0u;
+                            const uint32_t w = j0 >> 5, sh = j0 & 31u;
+                            auto word = [&](uint32_t i) { return i < prm.mask_words ? __ldg(mask + i) : 0u; };
+                            const uint32_t w0 = word(w), w1 = word(w + 1), w2 = word(w + 2);
+                            uint64_t see = static_cast<uint64_t>(__funnelshift_r(w0, w1, sh)) |
+                                           (static_cast<uint64_t>(__funnelshift_r(w1, w2, sh)) << 32);
+                            if (committed) see = (see << committed) | ((uint64_t(1) << committed) - 1);
+                            if (len - kv0 < kTreeTile) see &= (uint64_t(1) << (len - kv0)) - 1;
+                            const uint32_t see_lo = static_cast<uint32_t>(see), see_hi = static_cast<uint32_t>(see >> 32);
+#pragma unroll
+                            for (int c = 0; c < 32; ++c) {
+                                if (!((see_lo >> c) & 1u)) s[c] = 0xff800000u;        // -inf
+                                if (!((see_hi >> c) & 1u)) s[32 + c] = 0xff800000u;
+                            }
+                        }
+                        float alpha = 1.0f;
+                        if (moved) {
+                            float top = m_ref;   // fmaxf passes over NaN
+#pragma unroll
+                            for (int c = 0; c < 64; ++c) top = fmaxf(top, __uint_as_float(s[c]));
+                            if (top > m_ref + rescale_step || (m_ref == -INFINITY && top > -INFINITY)) {
+                                alpha = m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * scale);
+                                m_ref = top;
+                            }
+                            l_sum *= alpha;
+                        }
+                        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref * scale;
+                        const float2 scale2 = make_float2(scale, scale), neg_m2 = make_float2(neg_m, neg_m);
+                        float2 ps[2] = {};
+                        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float2 raw = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                            if (i & 1) t1 = max3(t1, raw.x, raw.y);
+                            else t0 = max3(t0, raw.x, raw.y);
+                            float2 x = fma2(raw, scale2, neg_m2);
+                            if (!EXACT && kFmaPairs * i % 32 < kFmaPairs) x = ex2_fma(x);
+                            else x = make_float2(ex2(x.x), ex2(x.y));
+                            ps[i & 1] = add2(ps[i & 1], x);
+                            const __half2 h = __float22half2_rn(x);
+                            hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                            if constexpr (EXACT) {
+                                const float2 back = __half22float2(h);
+                                lo[i] = pack(x.x - back.x, x.y - back.y);
+                            }
+                        }
+                        if (!moved) {
+                            const float top = max3(t0, t1, -INFINITY);
+                            if (__any_sync(0xffffffffu, !(top <= m_ref + rescale_step))) continue;
+                        } else if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                            where = 0x21;
+                            ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
+                            if (!ok) break;
+                            tc::fence_after();
+#pragma unroll 1
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t o[32];
+                                tc::tmem_ld32(tmem + lane_base + c0, o);
+                                tc::tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                tmem_st32(tmem + lane_base + c0, o);
+                            }
+                        }
+                        ps[0] = add2(ps[0], ps[1]);
+                        l_sum += ps[0].x + ps[0].y;
+                        break;
                     }
+                    if (!ok) break;
                     // P over this tile's scores (own lane, already read): the halves in 32 columns each
-                    tmem_st32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile, hi);
-                    if constexpr (EXACT) tmem_st32(tmem + lane_base + kTmemS + (g & 1u) * kTreeTile + 32, lo);
+                    tmem_st32(tS, hi);
+                    if constexpr (EXACT) tmem_st32(tS + 32, lo);
                     tmem_wait_st();
                 }
                 if (kv0 + kTreeTile > p.prefix) {
@@ -508,9 +558,9 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                     }
                     tc::fence_proxy_async_smem();
                 }
-                // Every warp follows pv_done phase by phase (a parity wait is only unambiguous for a waiter at most
-                // one phase behind). It costs nothing: P.V of this tile cannot start before the one before is done.
-                if (g > 0) {
+                // A parity wait for P.V of a tile needs the one before it to be done. For every other wait the tile's scores
+                // say so (they were issued behind it); the wait for the run's last P.V below has nothing in between.
+                if (j + 1 == p.n_tiles && g > 0) {
                     where = 0x24;
                     ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
                     if (!ok) break;
@@ -529,6 +579,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
             if (!ok) break;
             tc::fence_after();
+            if (l_sum < 1e-30f) l_sum = 0.f;   // a row that saw nothing: what ex2_fma leaves of -inf
             if (busy) {
                 const bool mine = row < done.n_rows;
                 const bool whole = done.slot == kTreeNoSlot;
@@ -607,7 +658,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const float* __restrict
     if (row >= rows) return;   // with WARPS > 1 a CTA has one row: all or none leave
     const TreeSplit sp = splits[row_split[row]];
     const uint32_t r = row - sp.first_row;
-    auto index = [&](uint32_t k) { return static_cast<size_t>(sp.first_slot + k) * slot_rows + r; };
+    auto index = [&](uint32_t k) { return static_cast<size_t>(sp.first_slot + k * sp.slot_step) * slot_rows + r; };
     float top = -INFINITY;
     for (uint32_t k = sub * 32 + lane; k < sp.n_parts; k += WARPS * 32) top = fmaxf(top, __ldcg(&part_ml[index(k)]).x);
 #pragma unroll

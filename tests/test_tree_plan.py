@@ -30,7 +30,7 @@ def work(tmp_path_factory):
         assert lib.tree_work(z(len(prefix)), z(H), z(KVH), ptr(prefix), ptr(draft), ptr(off), ctypes.c_uint32(max_ctas), ptr(pieces),
                              z(pieces.size), ptr(splits), z(splits.size), ptr(row_split), z(row_split.size), ptr(counts))
         n, ctas, ns, rows, slots, slot_rows = counts.tolist()
-        return (pieces[: 11 * n].reshape(n, 11).astype(np.int64), splits[: 7 * ns].reshape(ns, 7).astype(np.int64),
+        return (pieces[: 11 * n].reshape(n, 11).astype(np.int64), splits[: 8 * ns].reshape(ns, 8).astype(np.int64),
                 row_split[:rows], ctas, slots, slot_rows, off)
 
     return run
@@ -77,14 +77,24 @@ def test_every_tile_once(work, H, KVH, prefix, draft, max_ctas):
             if len(parts) == 1:
                 assert parts[0][2] == NO_SLOT and (unit[0], unit[1], row) not in by_split
                 continue
-            kv_head, r0, nr, t0, first, n_parts, first_row = by_split[(unit[0], unit[1], row)]
-            assert (nr, n_parts) == (n_rows, len(parts)) and [p[2] for p in parts] == list(range(first, first + n_parts))
+            kv_head, r0, nr, t0, first, n_parts, first_row, step = by_split[(unit[0], unit[1], row)]
+            assert (nr, n_parts) == (n_rows, len(parts)) and [p[2] for p in parts] == list(range(first, first + n_parts * step, step))
             index = [i for i, s in enumerate(splits.tolist()) if (s[3], s[0], s[1]) == (unit[0], unit[1], row)][0]
             assert (row_split[first_row: first_row + nr] == index).all()
             used += [p[2] for p in parts]
             merged += nr
         assert at == rows
     assert sorted(used) == list(range(slots)) and merged == len(row_split)
+
+
+def test_row_tiles_of_a_unit_run_side_by_side(work):
+    """CTAs of one group have the same runs: what one of them reads from memory, the others find in L2."""
+    pieces, *_, ctas, slots, slot_rows, off = work(32, 8, [3000, 900, 4000] * 5, [64, 7, 33] * 5, 296)
+    runs = {}
+    for cta, h, row, n_rows, begin, n, slot, c, d, t0, pt in pieces.tolist():
+        runs.setdefault((t0, h, begin, n), []).append(cta)
+    for (t0, h, begin, n), group in runs.items():
+        assert max(group) - min(group) == len(group) - 1
 
 
 def test_runs_are_even(work):

@@ -4,7 +4,7 @@
 #include <cstring>
 
 // out: per piece {cta, kv_head, row_begin, n_rows, tile_begin, n_tiles, slot, prefix, draft, token0, pt_off}; splits: per split
-// {kv_head, row_begin, n_rows, token0, first_slot, n_parts, first_row}; counts: {pieces, ctas, splits, merged rows, slots, slot rows}.
+// {kv_head, row_begin, n_rows, token0, first_slot, n_parts, first_row, slot_step}; counts: {pieces, ctas, splits, merged rows, slots, slot rows}.
 extern "C" int tree_work(size_t batch, size_t H, size_t KVH, const uint32_t* prefix, const uint32_t* draft, const uint32_t* pt_off,
                          uint32_t max_ctas, uint32_t* out, size_t out_words, uint32_t* splits, size_t split_words, uint32_t* row_split,
                          size_t row_words, uint32_t* counts) {
@@ -18,7 +18,7 @@ extern "C" int tree_work(size_t batch, size_t H, size_t KVH, const uint32_t* pre
     t.pt_off = pt_off;
     mlcb::TreeWork w;
     mlcb::tree_work_list(s, t, max_ctas, &w);
-    if (w.pieces.size() * 11 > out_words || w.splits.size() * 7 > split_words || w.row_split.size() > row_words) return 0;
+    if (w.pieces.size() * 11 > out_words || w.splits.size() * 8 > split_words || w.row_split.size() > row_words) return 0;
     for (size_t c = 0; c + 1 < w.cta_off.size(); ++c)
         for (uint32_t i = w.cta_off[c]; i < w.cta_off[c + 1]; ++i) {
             const mlcb::TreePiece& p = w.pieces[i];
@@ -28,8 +28,8 @@ extern "C" int tree_work(size_t batch, size_t H, size_t KVH, const uint32_t* pre
         }
     for (size_t i = 0; i < w.splits.size(); ++i) {
         const mlcb::TreeSplit& p = w.splits[i];
-        const uint32_t v[7] = {p.kv_head, p.row_begin, p.n_rows, p.token0, p.first_slot, p.n_parts, p.first_row};
-        std::memcpy(splits + 7 * i, v, sizeof(v));
+        const uint32_t v[8] = {p.kv_head, p.row_begin, p.n_rows, p.token0, p.first_slot, p.n_parts, p.first_row, p.slot_step};
+        std::memcpy(splits + 8 * i, v, sizeof(v));
     }
     if (!w.row_split.empty()) std::memcpy(row_split, w.row_split.data(), w.row_split.size() * 4);
     const uint32_t n[6] = {static_cast<uint32_t>(w.pieces.size()), static_cast<uint32_t>(w.cta_off.size() - 1),

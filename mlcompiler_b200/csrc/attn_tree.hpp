@@ -34,7 +34,7 @@ struct TreePiece {
     uint32_t tile_begin, n_tiles;
     uint32_t slot;                         // where the partial goes; kTreeNoSlot: the piece is the whole run
     uint32_t prefix, draft, token0, pt_off;
-    uint32_t pad[2];
+    uint32_t more, next;                   // first piece of a CTA: it has `more` others, from pieces[next] on
 };
 static_assert(sizeof(TreePiece) == 48, "read as three 16-byte vectors");
 
@@ -45,8 +45,8 @@ struct TreeSplit {
 static_assert(sizeof(TreeSplit) == 32, "read as two 16-byte vectors");
 
 struct TreeWork {
-    std::vector<TreePiece> pieces;
-    std::vector<uint32_t> cta_off;    // pieces of CTA c: [cta_off[c], cta_off[c + 1])
+    std::vector<TreePiece> pieces;    // the first piece of every CTA, then the others, CTA by CTA
+    uint32_t n_cta = 0;
     std::vector<TreeSplit> splits;
     std::vector<uint32_t> row_split;  // split of every merged row
     uint32_t n_slots = 0, slot_rows = 0;
@@ -57,7 +57,6 @@ struct TreeView {   // device addresses inside one image
     const uint32_t *token0 = nullptr;     // first drafted token of a request in q / o, [batch + 1]
     const uint32_t *token_req = nullptr;  // request of a drafted token
     const TreePiece* pieces = nullptr;
-    const uint32_t* cta_off = nullptr;
     const TreeSplit* splits = nullptr;
     const uint32_t* row_split = nullptr;
     uint32_t n_cta = 0, n_slots = 0, slot_rows = 0, merge_rows = 0;

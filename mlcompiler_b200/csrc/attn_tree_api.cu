@@ -32,7 +32,7 @@ size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 
 // Offsets of an image's parts.
 struct TreeLayout {
-    size_t flat, off, prefix, draft, token0, token_req, mask, pieces, cta_off, splits, row_split, total;
+    size_t flat, off, prefix, draft, token0, token_req, mask, pieces, splits, row_split, total;
 };
 
 TreeLayout layout_of(const TreeShape& s, const TreeWork& w) {
@@ -45,7 +45,6 @@ TreeLayout layout_of(const TreeShape& s, const TreeWork& w) {
     };
     l.pieces = take(w.pieces.size() * sizeof(TreePiece));
     l.splits = take(w.splits.size() * sizeof(TreeSplit));
-    l.cta_off = take(w.cta_off.size() * 4);
     l.row_split = take(w.row_split.size() * 4);
     l.flat = take(s.n_flat * 4);
     l.off = take((s.batch + 1) * 4);
@@ -65,7 +64,6 @@ void put(uint8_t* at, const void* src, size_t bytes) {
 void fill_image(uint8_t* h, const TreeLayout& l, const TreeShape& s, const TreeTables& t, const TreeWork& w) {
     put(h + l.pieces, w.pieces.data(), w.pieces.size() * sizeof(TreePiece));
     put(h + l.splits, w.splits.data(), w.splits.size() * sizeof(TreeSplit));
-    put(h + l.cta_off, w.cta_off.data(), w.cta_off.size() * 4);
     put(h + l.row_split, w.row_split.data(), w.row_split.size() * 4);
     put(h + l.flat, t.pt_flat, s.n_flat * 4);
     put(h + l.off, t.pt_off, (s.batch + 1) * 4);
@@ -93,10 +91,9 @@ TreeView view_of(const uint8_t* dev, const TreeLayout& l, const TreeWork& w) {
     v.token_req = words(l.token_req);
     v.mask = words(l.mask);
     v.pieces = reinterpret_cast<const TreePiece*>(dev + l.pieces);
-    v.cta_off = words(l.cta_off);
     v.splits = reinterpret_cast<const TreeSplit*>(dev + l.splits);
     v.row_split = words(l.row_split);
-    v.n_cta = w.cta_off.empty() ? 0u : static_cast<uint32_t>(w.cta_off.size() - 1);
+    v.n_cta = w.n_cta;
     v.n_slots = w.n_slots;
     v.slot_rows = w.slot_rows;
     v.merge_rows = static_cast<uint32_t>(w.row_split.size());

@@ -27,8 +27,7 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
     out->pieces.clear();
     out->splits.clear();
     out->row_split.clear();
-    out->cta_off.assign(1, 0);
-    out->n_slots = out->slot_rows = 0;
+    out->n_cta = out->n_slots = out->slot_rows = 0;
     const uint32_t G = static_cast<uint32_t>(s.H / s.KVH);
     // Row tiles side by side, at most: beyond, they share a run through L2 in turns. One where there are too few CTAs for
     // a group of every width.
@@ -69,19 +68,18 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
         token0 += draft;
     }
     if (total == 0 || max_ctas == 0) return;
-    uint64_t quota = std::max<uint64_t>((total + max_ctas - 1) / max_ctas, kMinPiece + kPieceCost);
+    std::vector<std::vector<TreePiece>> ctas;
+    uint64_t quota = std::max<uint64_t>((total + max_ctas - 1) / max_ctas, kPieceCost + 1);
     for (;; quota += quota / 32 + 1) {   // rounding at the cuts may need a CTA more than there are: try again with longer runs
-        out->pieces.clear();
+        ctas.clear();
         out->splits.clear();
         out->row_split.clear();
-        out->cta_off.assign(1, 0);
         out->n_slots = 0;
         std::vector<std::vector<TreePiece>> group;   // pieces of the CTAs of the current group
         uint64_t used = 0;
         auto close_group = [&] {
             for (auto& lane : group) {
-                out->pieces.insert(out->pieces.end(), lane.begin(), lane.end());
-                out->cta_off.push_back(static_cast<uint32_t>(out->pieces.size()));
+                ctas.push_back(std::move(lane));
                 lane.clear();
             }
             used = 0;
@@ -94,7 +92,7 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
                 const uint32_t first_slot = out->n_slots;
                 while (at < u.tiles) {
                     if (used && used + kPieceCost + std::min(kMinPiece, u.tiles - at) > quota) close_group();
-                    const uint64_t room = quota - used - kPieceCost;   // >= the smallest piece, see the quota's lower bound
+                    const uint64_t room = std::max<uint64_t>(quota - used - kPieceCost, kMinPiece);
                     uint32_t take = static_cast<uint32_t>(std::min<uint64_t>(u.tiles - at, room));
                     if (u.tiles - at - take < kMinPiece) take = u.tiles - at;
                     const bool cut = at || take < u.tiles;
@@ -129,8 +127,17 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
             }
             if (used) close_group();
         }
-        if (out->cta_off.size() - 1 <= max_ctas) return;
+        if (ctas.size() <= max_ctas) break;
     }
+    out->n_cta = static_cast<uint32_t>(ctas.size());
+    uint32_t next = out->n_cta;
+    for (const auto& c : ctas) {
+        out->pieces.push_back(c.front());
+        out->pieces.back().more = static_cast<uint32_t>(c.size() - 1);
+        out->pieces.back().next = next;
+        next += static_cast<uint32_t>(c.size() - 1);
+    }
+    for (const auto& c : ctas) out->pieces.insert(out->pieces.end(), c.begin() + 1, c.end());
 }
 
 }  // namespace mlcb

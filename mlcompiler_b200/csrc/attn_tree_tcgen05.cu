@@ -5,9 +5,9 @@
 // tokens and a group of 8 they fill the 128 rows of the tensor core's tile, and every K / V tile is read once for all of
 // them. Per 64 tokens of the cache:
 //   S[128x64]  = Q[128xD] . K^T       A and B from shared memory, fp32 accumulator in tensor memory
-//   softmax    : thread t owns row t; running maximum and sum in fp32, base-2 exponentials, P rounded to fp16 back into
-//                tensor memory as the next A operand. The output is rescaled only when a row's maximum has grown by
-//                more than 2^8 since the last rescale (exact: P <= 256, and the final 1 / l uses the same reference)
+//   softmax    : thread t owns row t; reference maximum and sum in fp32, base-2 exponentials, P rounded to fp16 back into
+//                tensor memory as the next A operand. The reference is the maximum of the run's first tile and moves up
+//                only when the weights outgrow fp16 (exact: the final 1 / l uses the same reference)
 //   O[128xD] += P[128x64] . V
 // The tree mask only matters in the tiles that hold drafted tokens, the last ones of a request: there a row's 64 mask
 // bits are cut out of its mask words. In those tiles V is also searched for infinities and NaN - a masked token has
@@ -37,20 +37,26 @@ namespace {
 
 constexpr uint32_t kSlabQ = kTreeRows * 128;   // 64 halfs of every query row
 constexpr uint32_t kSlabKV = kTreeTile * 128;  // 64 halfs of every token of a tile
-constexpr uint32_t kTmemCols = 256;            // O: up to 128 columns, S: 2 x 64
+constexpr uint32_t kTmemCols = 256;            // O: up to 128 columns, S: 2 x 64; D = 64: Q behind O
 constexpr uint32_t kTmemS = 128;
+constexpr uint32_t kTmemQ = 64;
 constexpr uint32_t kThreads = 224;
+constexpr uint32_t kStageBytes = 32 * 128;     // per softmax warp: 128 bytes of each of its rows, on the way in or out
 constexpr int kFmaPairs = 12;                  // of a tile's 32 pairs of columns: exponentials on the FMA pipe
 
 template <int D, bool EXACT>
 struct Config {
     static constexpr uint32_t slabs = D / 64;
-    static constexpr uint32_t q_bytes = slabs * kSlabQ * (EXACT ? 2 : 1);
+    // Q as an operand in tensor memory where there is room beside O and S: read from shared memory, its 128 rows cost
+    // every product twice what the 64 rows of K do
+    static constexpr bool q_tmem = D == 64;
+    static constexpr uint32_t q_bytes = q_tmem ? 0 : slabs * kSlabQ * (EXACT ? 2 : 1);
     static constexpr uint32_t kv_bytes = slabs * kSlabKV;   // one tile of K, or of V
     // two CTAs per SM share 226 KB; with D = 128 the two halves of Q leave room for one CTA only
     static constexpr uint32_t ctas = EXACT && D == 128 ? 1 : 2;
-    static constexpr uint32_t stages = EXACT ? 4 : (D == 128 ? 2 : 5);
+    static constexpr uint32_t stages = D == 64 ? 6 : EXACT ? 4 : 2;
     static constexpr uint32_t tile_bytes = q_bytes + stages * 2 * kv_bytes;
+    static constexpr uint32_t smem_bytes = tile_bytes + 4 * kStageBytes;   // and the barriers behind that
 };
 
 template <uint32_t STAGES>
@@ -66,7 +72,7 @@ struct TreeParams {
     float* part_o;    // [slot][slot_rows][D]
     float2* part_ml;  // [slot][slot_rows] (reference maximum in base-2 units, sum)
     const TreePiece* pieces;
-    const uint32_t *cta_off, *pt_flat, *mask;
+    const uint32_t *pt_flat, *mask;
     uint32_t* err;
     uint32_t H, KVH, G, P, mask_words, slot_rows;
     uint32_t box_rows, boxes;   // TMA boxes of a tile: boxes * box_rows = 64
@@ -80,12 +86,6 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-// NaN if one of the three is.
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
 }
 // Two fp32 operations in one instruction, on register pairs.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -148,6 +148,10 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
+__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -176,26 +180,86 @@ __device__ __forceinline__ TreePiece load_piece(const TreePiece* p) {
 // Bit 15 / 31 of the result: the lower / upper fp16 of w is infinite or NaN.
 __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
 
-// Puts query row `row` (or zeros) into the swizzled operand tile(s); returns what the scores have to be multiplied with
-// to undo the row's scaling.
-template <int D, bool EXACT>
-__device__ __forceinline__ float load_query_row(uint32_t sQ, uint32_t row, const void* q, int q_f32, bool valid, size_t elem) {
-    const uint32_t base = sQ + (row >> 3) * 1024u + (row & 7u) * 128u;
-    auto at = [&](uint32_t c) { return base + (c >> 3) * kSlabQ + (((c ^ row) & 7u) << 4); };
-    if constexpr (!EXACT) {
-        const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __half*>(q) + elem);
+// Rows of q and o lie a token apart or a head apart; a thread that moves its own row touches 32 lines per instruction and warp.
+// The warp moves 128 bytes of four rows at a time instead, eight lanes a row, by way of shared memory, where a thread finds
+// its own row. 16-byte chunk c of row r sits at r * 128 + ((c ^ r) & 7) * 16.
+__device__ __forceinline__ uint32_t staged(uint32_t stage, uint32_t r, uint32_t c) { return stage + r * 128 + (((c ^ r) & 7u) << 4); }
+
+// 128 bytes, from byte `offset` of this lane's row on (rows of invalid lanes: zeros), to shared memory.
+__device__ __forceinline__ void stage_in(uint32_t stage, uint32_t lane, const char* row, bool valid, uint32_t offset) {
+    const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+    const uint64_t mine = reinterpret_cast<uint64_t>(row + offset);
+    uint4 v[8];
 #pragma unroll
-        for (uint32_t c = 0; c < D / 8; ++c) st_shared16(at(c), valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0));
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t r = 4 * i + (lane >> 3);
+        const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, mine, r));
+        v[i] = (rows >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(src) + (lane & 7u)) : make_uint4(0, 0, 0, 0);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) st_shared16(staged(stage, 4 * i + (lane >> 3), lane & 7u), v[i]);
+    __syncwarp();
+}
+
+// The reverse: w is 128 bytes of this lane's row.
+__device__ __forceinline__ void stage_out(uint32_t stage, uint32_t lane, char* row, bool valid, uint32_t offset, const uint32_t (&w)[32]) {
+    const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+    const uint64_t mine = reinterpret_cast<uint64_t>(row + offset);
+    __syncwarp();
+#pragma unroll
+    for (int c = 0; c < 8; ++c) st_shared16(staged(stage, lane, c), make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]));
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t r = 4 * i + (lane >> 3);
+        char* dst = reinterpret_cast<char*>(__shfl_sync(0xffffffffu, mine, r));
+        if ((rows >> r) & 1u) reinterpret_cast<uint4*>(dst)[lane & 7u] = ld_shared16(staged(stage, r, lane & 7u));
+    }
+}
+
+// Puts the warp's query rows (zeros for invalid lanes) into the operand tile(s), in shared memory (swizzled) or in tensor
+// memory; returns what the lane's scores have to be multiplied with to undo its row's scaling.
+template <int D, bool EXACT>
+__device__ __forceinline__ float load_queries(uint32_t sQ, uint32_t tQ, uint32_t stage, uint32_t row, const void* q, int q_f32, bool valid,
+                                              size_t elem) {
+    constexpr bool TMEM = Config<D, EXACT>::q_tmem;
+    const uint32_t lane = row & 31u;
+    const uint32_t base = sQ + (row >> 3) * 1024u + (row & 7u) * 128u;
+    auto to_shared = [&](uint32_t half, uint32_t c, const uint32_t* w) {   // 16 bytes
+        st_shared16(base + (half * (D / 64) + (c >> 3)) * kSlabQ + (((c ^ row) & 7u) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+    };
+    const char* src = static_cast<const char*>(q) + elem * (q_f32 ? 4 : 2);
+    if constexpr (!EXACT) {
+#pragma unroll
+        for (int block = 0; block < D / 64; ++block) {   // 64 halfs
+            stage_in(stage, lane, src, valid, block * 128);
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const uint4 v = ld_shared16(staged(stage, lane, c));
+                w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+            }
+            if constexpr (TMEM) {
+                tmem_st32(tQ, w);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) to_shared(0, block * 8 + c, w + 4 * c);
+            }
+        }
+        if constexpr (TMEM) tmem_wait_st();
         return 1.0f;
     } else {
-        auto load8 = [&](uint32_t c, float (&x)[8]) {
+        // 8 columns of the lane's row out of the block of 32 (fp32) or 64 (fp16) that is staged
+        auto read8 = [&](uint32_t c, float (&x)[8]) {
             if (q_f32) {
-                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(q) + elem) + 2 * c;
-                const float4 a = __ldg(src), b = __ldg(src + 1);
-                x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+                const uint4 a = ld_shared16(staged(stage, lane, 2 * c)), b = ld_shared16(staged(stage, lane, 2 * c + 1));
+                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
             } else {
-                const uint4 v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __half*>(q) + elem) + c);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                const uint4 a = ld_shared16(staged(stage, lane, c));
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
@@ -203,12 +267,14 @@ __device__ __forceinline__ float load_query_row(uint32_t sQ, uint32_t row, const
                 }
             }
         };
+        const uint32_t per_block = q_f32 ? 4 : 8, blocks = D / 8 / per_block;   // groups of 8 columns
         float top = 0.f;
-        if (valid) {
-#pragma unroll 4
-            for (uint32_t c = 0; c < D / 8; ++c) {
+        for (uint32_t k = 0; k < blocks; ++k) {
+            stage_in(stage, lane, src, valid, k * 128);
+#pragma unroll 2
+            for (uint32_t c = 0; c < per_block; ++c) {
                 float x[8];
-                load8(c, x);
+                read8(c, x);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
             }
@@ -217,22 +283,32 @@ __device__ __forceinline__ float load_query_row(uint32_t sQ, uint32_t row, const
         int shift = 0;
         if (top > 0.f && top < INFINITY) shift = max(-120, min(120, 7 - ilogbf(top)));
         const float up = __int_as_float((127 + shift) << 23), down = __int_as_float((127 - shift) << 23);
-#pragma unroll 4
-        for (uint32_t c = 0; c < D / 8; ++c) {
-            float x[8] = {};
-            if (valid) load8(c, x);
-            uint32_t hi[4], lo[4];
+        for (uint32_t k = 0; k < blocks; ++k) {
+            stage_in(stage, lane, src, valid, k * 128);
+#pragma unroll 2
+            for (uint32_t c = 0; c < per_block; ++c) {
+                float x[8];
+                read8(c, x);
+                uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
-                const __half2 h = __floats2half2_rn(a, b);
-                const float2 back = __half22float2(h);
-                hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                lo[i] = pack(a - back.x, b - back.y);
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+                    const __half2 h = __floats2half2_rn(a, b);
+                    const float2 back = __half22float2(h);
+                    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                    lo[i] = pack(a - back.x, b - back.y);
+                }
+                const uint32_t at = k * per_block + c;
+                if constexpr (TMEM) {
+                    tmem_st4(tQ + 4 * at, hi);
+                    tmem_st4(tQ + D / 2 + 4 * at, lo);
+                } else {
+                    to_shared(0, at, hi);
+                    to_shared(1, at, lo);
+                }
             }
-            st_shared16(at(c), make_uint4(hi[0], hi[1], hi[2], hi[3]));
-            st_shared16(at(c) + (D / 64) * kSlabQ, make_uint4(lo[0], lo[1], lo[2], lo[3]));
         }
+        if constexpr (TMEM) tmem_wait_st();
         return down;
     }
 }
@@ -244,7 +320,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     using C = Config<D, EXACT>;
     constexpr uint32_t STAGES = C::stages;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    Bars<STAGES>& bars = *reinterpret_cast<Bars<STAGES>*>(smem_raw + C::tile_bytes);
+    Bars<STAGES>& bars = *reinterpret_cast<Bars<STAGES>*>(smem_raw + C::smem_bytes);
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t base = smem_u32(smem_raw);
     if (base & 1023u) {   // the swizzle needs it; never expected
@@ -273,10 +349,12 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = bars.tmem_slot;
+    // The work list and the page tables were uploaded before the kernel in front was launched, and no kernel writes them:
+    // they are read before the wait for that kernel.
+    TreePiece p = load_piece(prm.pieces + blockIdx.x);
+    const uint32_t n_pieces = 1 + p.more, next_piece = p.next;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    const uint32_t first = __ldg(prm.cta_off + blockIdx.x), last = __ldg(prm.cta_off + blockIdx.x + 1);
     // A wait that ran out: which wait (bits 8-15 of the error word) and at which tile (bits 16-31).
     auto give_up = [&](uint32_t where, uint32_t tile) {
         if (lane == 0 && atomicCAS(prm.err, 0u, MLC_DEVERR_WAIT_TIMEOUT | (where << 8) | (tile << 16)) != 0u)
@@ -291,15 +369,21 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
         uint64_t* full = is_v ? bars.v_full : bars.k_full;
         uint64_t* empty = is_v ? bars.v_empty : bars.k_empty;
         const uint32_t ring = sKV + (is_v ? C::kv_bytes : 0u);
+        if (lane == 0) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
         uint32_t g = 0;   // tiles of this CTA so far
         bool ok = true;
-        for (uint32_t pi = first; ok && pi < last; ++pi) {
-            const TreePiece p = load_piece(prm.pieces + pi);
+        for (uint32_t pi = 0; ok && pi < n_pieces; ++pi) {
+            if (pi) p = load_piece(prm.pieces + next_piece + pi - 1);
             const uint32_t len = p.prefix + p.draft;
             const uint32_t token_begin = p.tile_begin * kTreeTile;
             // boxes of the piece that hold tokens; their page ids are fetched 32 at a time, a lane each
             const uint32_t n_boxes = (min(len, token_begin + p.n_tiles * kTreeTile) - token_begin + prm.box_rows - 1) / prm.box_rows;
-            uint32_t box = 0, ids = 0;
+            auto fetch_ids = [&](uint32_t box) {
+                const uint32_t mine = box + lane;
+                return mine < n_boxes ? __ldg(prm.pt_flat + p.pt_off + (token_begin + mine * prm.box_rows) / prm.P) : 0u;
+            };
+            uint32_t box = 0, ids = fetch_ids(0);
+            if (pi == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
             for (uint32_t j = 0; j < p.n_tiles; ++j, ++g) {
                 const uint32_t s = g % STAGES;
                 if (g >= STAGES && !warp_wait(smem_u32(&empty[s]), (g / STAGES - 1) & 1u)) {
@@ -311,10 +395,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 const uint32_t bar = smem_u32(&full[s]), dst = ring + s * 2 * C::kv_bytes;
                 if (lane == 0) expect_tx(bar, in_tile * prm.box_rows * D * 2);
                 for (uint32_t b = 0; b < in_tile; ++b, ++box) {
-                    if ((box & 31u) == 0) {
-                        const uint32_t mine = box + lane;
-                        ids = mine < n_boxes ? __ldg(prm.pt_flat + p.pt_off + (token_begin + mine * prm.box_rows) / prm.P) : 0u;
-                    }
+                    if (box && (box & 31u) == 0) ids = fetch_ids(box);
                     const int page = static_cast<int>(__shfl_sync(0xffffffffu, ids, box & 31u));
                     const int slot = static_cast<int>((token_begin + box * prm.box_rows) % prm.P);
                     if (lane == 0) {
@@ -345,9 +426,13 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 for (uint32_t half = 0; half < (EXACT ? 2u : 1u); ++half)
 #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k) {
-                        const uint32_t a = sQ_u + (half * C::slabs + (k >> 2)) * kSlabQ + (k & 3) * 32;
                         const uint32_t b = sK + (k >> 2) * kSlabKV + (k & 3) * 32;
-                        tc::mma_f16(d, desc_k | (a >> 4), desc_k | (b >> 4), idesc_qk, half + k > 0);
+                        if constexpr (C::q_tmem) {
+                            mma_f16_ts(d, tmem_u + kTmemQ + half * 32 + k * 8, desc_k | (b >> 4), idesc_qk, half + k > 0);
+                        } else {
+                            const uint32_t a = sQ_u + (half * C::slabs + (k >> 2)) * kSlabQ + (k & 3) * 32;
+                            tc::mma_f16(d, desc_k | (a >> 4), desc_k | (b >> 4), idesc_qk, half + k > 0);
+                        }
                     }
                 tc::commit(smem_u32(&bars.k_empty[s]));
                 tc::commit(smem_u32(&bars.s_full[g & 1u]));
@@ -370,9 +455,10 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             issued_qk = t + 1;
             return true;
         };
-        for (uint32_t pi = first; ok && pi < last; ++pi) {
-            const uint32_t n_tiles = __ldg(&prm.pieces[pi].n_tiles);
-            if (!all_wait(&bars.q_full, (pi - first) & 1u, 0x10) || !start_tile(g)) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        for (uint32_t pi = 0; ok && pi < n_pieces; ++pi) {
+            const uint32_t n_tiles = pi ? __ldg(&prm.pieces[next_piece + pi - 1].n_tiles) : p.n_tiles;
+            if (!all_wait(&bars.q_full, pi & 1u, 0x10) || !start_tile(g)) {
                 ok = false;
                 break;
             }
@@ -411,22 +497,23 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
         uint32_t g = 0, where = 0x20;
         bool ok = true;
         float row_down = 1.0f;
-        TreePiece p = load_piece(prm.pieces + first);
+        const uint32_t stage = base + C::tile_bytes + warp * kStageBytes;
         auto put_query = [&](const TreePiece& pc) {
             const uint32_t r = pc.row_begin + row;
             const size_t elem = (static_cast<size_t>(pc.token0 + r / prm.G) * prm.H + pc.kv_head * prm.G + r % prm.G) * D;
-            row_down = load_query_row<D, EXACT>(sQ, row, prm.q, prm.q_f32, row < pc.n_rows, elem);
-            tc::fence_proxy_async_smem();
+            row_down = load_queries<D, EXACT>(sQ, tmem + lane_base + kTmemQ, stage, row, prm.q, prm.q_f32, row < pc.n_rows, elem);
+            if constexpr (C::q_tmem) tc::fence_before();
+            else tc::fence_proxy_async_smem();
             tc::mbar_arrive(smem_u32(&bars.q_full));
         };
-        if (first < last) put_query(p);
-        for (uint32_t pi = first; ok && pi < last; ++pi) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        put_query(p);
+        for (uint32_t pi = 0; ok && pi < n_pieces; ++pi) {
             const uint32_t len = p.prefix + p.draft;
             const bool busy = warp * 32u < p.n_rows;   // the warp has rows
             const uint32_t r = p.row_begin + min(row, p.n_rows - 1);
             const uint32_t* mask = prm.mask + static_cast<size_t>(p.token0 + r / prm.G) * prm.mask_words;
             const float scale = prm.scale_log2 * row_down;      // of a raw score, base-2 units
-            const float rescale_step = 8.0f / scale;
             float m_ref = -INFINITY, l_sum = 0.f;               // reference maximum (raw scores) of the accumulator, row sum
             for (uint32_t j = 0; j < p.n_tiles; ++j, ++g) {
                 const uint32_t kv0 = (p.tile_begin + j) * kTreeTile;
@@ -437,9 +524,9 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 if (busy) {
                     const uint32_t tS = tmem + lane_base + kTmemS + (g & 1u) * kTreeTile;
                     uint32_t hi[32], lo[EXACT ? 32 : 1];
-                    // First with the reference maximum as it is: the exponentials need not wait for the tile's maximum, which
-                    // is found beside them. Where some row's maximum has outgrown its reference (or is NaN), and on a run's
-                    // first tile, the tile is done (again) with a new reference.
+                    // First with the reference maximum as it is, without looking for the tile's: every weight is below the
+                    // row's sum over the tile, and while that is below 2^15 the weights fit fp16. Where some row's sum is not
+                    // (or is NaN), and on a run's first tile, the tile is done (again) with a new reference.
                     for (bool moved = j == 0;; moved = true) {
                         uint32_t s[64];
                         {
@@ -473,7 +560,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                             float top = m_ref;   // fmaxf passes over NaN
 #pragma unroll
                             for (int c = 0; c < 64; ++c) top = fmaxf(top, __uint_as_float(s[c]));
-                            if (top > m_ref + rescale_step || (m_ref == -INFINITY && top > -INFINITY)) {
+                            if (top > m_ref) {
                                 alpha = m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * scale);
                                 m_ref = top;
                             }
@@ -482,12 +569,9 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                         const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref * scale;
                         const float2 scale2 = make_float2(scale, scale), neg_m2 = make_float2(neg_m, neg_m);
                         float2 ps[2] = {};
-                        float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const float2 raw = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                            if (i & 1) t1 = max3(t1, raw.x, raw.y);
-                            else t0 = max3(t0, raw.x, raw.y);
                             float2 x = fma2(raw, scale2, neg_m2);
                             if (!EXACT && kFmaPairs * i % 32 < kFmaPairs) x = ex2_fma(x);
                             else x = make_float2(ex2(x.x), ex2(x.y));
@@ -499,9 +583,11 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                                 lo[i] = pack(x.x - back.x, x.y - back.y);
                             }
                         }
+                        ps[0] = add2(ps[0], ps[1]);
+                        const float sum = ps[0].x + ps[0].y;
                         if (!moved) {
-                            const float top = max3(t0, t1, -INFINITY);
-                            if (__any_sync(0xffffffffu, !(top <= m_ref + rescale_step))) continue;
+                            // (a reference of -inf is none)
+                            if (__any_sync(0xffffffffu, !(sum < 32768.0f) || m_ref == -INFINITY)) continue;
                         } else if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                             where = 0x21;
                             ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
@@ -517,8 +603,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                                 tmem_st32(tmem + lane_base + c0, o);
                             }
                         }
-                        ps[0] = add2(ps[0], ps[1]);
-                        l_sum += ps[0].x + ps[0].y;
+                        l_sum += sum;
                         break;
                     }
                     if (!ok) break;
@@ -571,8 +656,8 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             if (!ok) break;
             // every Q.K^T of this piece is done: the next one's queries may move in while the last P.V runs
             const TreePiece done = p;
-            if (pi + 1 < last) {
-                p = load_piece(prm.pieces + pi + 1);
+            if (pi + 1 < n_pieces) {
+                p = load_piece(prm.pieces + next_piece + pi);
                 put_query(p);
             }
             where = 0x23;
@@ -588,48 +673,42 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 const size_t part = static_cast<size_t>(done.slot) * prm.slot_rows + row;
                 const bool repair = *reinterpret_cast<volatile uint32_t*>(&bars.not_finite) == pi + 1;
                 if (!whole && mine) prm.part_ml[part] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * scale, l_sum);
-#pragma unroll 1
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(tmem + lane_base + c0, o);
-                    tc::tmem_wait_ld();
-                    if (!mine) continue;
-                    if (repair) {
-                        // drafted tokens of this piece that the row sees: what is not finite in V belongs in its output
-                        const uint32_t begin = done.tile_begin * kTreeTile, stop = min(len, begin + done.n_tiles * kTreeTile);
-                        for (uint32_t pos = max(begin, done.prefix); pos < stop; ++pos) {
-                            const uint32_t t = pos - done.prefix;
-                            if (!((__ldg(mask + (t >> 5)) >> (t & 31u)) & 1u)) continue;
-                            const size_t page = __ldg(prm.pt_flat + done.pt_off + pos / prm.P);
-                            const __half* v = prm.v_pages + ((page * prm.P + pos % prm.P) * prm.KVH + done.kv_head) * D + c0;
+                // drafted tokens of this piece that the row sees: what is not finite in V belongs in its output
+                auto put_back = [&](int c0, uint32_t (&o)[32]) {
+                    const uint32_t begin = done.tile_begin * kTreeTile, stop = min(len, begin + done.n_tiles * kTreeTile);
+                    for (uint32_t pos = max(begin, done.prefix); pos < stop; ++pos) {
+                        const uint32_t t = pos - done.prefix;
+                        if (!((__ldg(mask + (t >> 5)) >> (t & 31u)) & 1u)) continue;
+                        const size_t page = __ldg(prm.pt_flat + done.pt_off + pos / prm.P);
+                        const __half* v = prm.v_pages + ((page * prm.P + pos % prm.P) * prm.KVH + done.kv_head) * D + c0;
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) {
-                                const float x = __half2float(v[i]);
-                                if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
-                            }
+                        for (int i = 0; i < 32; ++i) {
+                            const float x = __half2float(v[i]);
+                            if (!(fabsf(x) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + x);
                         }
                     }
-                    if (!whole) {
-                        float4* dst = reinterpret_cast<float4*>(prm.part_o + part * D + c0);
+                };
+                const bool wide = !whole || prm.o_f32;   // 4 bytes a column leave, or 2
+                char* dst = whole ? static_cast<char*>(prm.o) + out * (prm.o_f32 ? 4 : 2) : reinterpret_cast<char*>(prm.part_o + part * D);
+#pragma unroll 1
+                for (int c0 = 0; c0 < D; c0 += 64) {
+                    uint32_t w[32];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            dst[i] = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]),
-                                                 __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
-                    } else if (prm.o_f32) {
-                        float4* dst = reinterpret_cast<float4*>(static_cast<float*>(prm.o) + out + c0);
+                    for (int half = 0; half < 2; ++half) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(tmem + lane_base + c0 + 32 * half, o);
+                        tc::tmem_wait_ld();
+                        if (repair && mine) put_back(c0 + 32 * half, o);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv, __uint_as_float(o[4 * i + 1]) * inv,
-                                                 __uint_as_float(o[4 * i + 2]) * inv, __uint_as_float(o[4 * i + 3]) * inv);
-                    } else {
-                        uint4* dst = reinterpret_cast<uint4*>(static_cast<__half*>(prm.o) + out + c0);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+                        if (wide) {
+                            stage_out(stage, lane, dst, mine, (c0 + 32 * half) * 4, o);
+                        } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            dst[i] = make_uint4(pack(__uint_as_float(o[8 * i]) * inv, __uint_as_float(o[8 * i + 1]) * inv),
-                                                pack(__uint_as_float(o[8 * i + 2]) * inv, __uint_as_float(o[8 * i + 3]) * inv),
-                                                pack(__uint_as_float(o[8 * i + 4]) * inv, __uint_as_float(o[8 * i + 5]) * inv),
-                                                pack(__uint_as_float(o[8 * i + 6]) * inv, __uint_as_float(o[8 * i + 7]) * inv));
+                            for (int i = 0; i < 16; ++i) w[16 * half + i] = pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+                        }
                     }
+                    if (!wide) stage_out(stage, lane, dst, mine, c0 * 2, w);
                 }
             }
         }
@@ -748,7 +827,7 @@ cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, co
 template <int D, bool EXACT>
 int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a) {
     using C = Config<D, EXACT>;
-    constexpr size_t smem = C::tile_bytes + sizeof(Bars<C::stages>);
+    constexpr size_t smem = C::smem_bytes + sizeof(Bars<C::stages>);
     const uint32_t box_rows = static_cast<uint32_t>(s.P < kTreeTile ? s.P : kTreeTile);
     CUtensorMap mk, mv;
     int st = pool_map(ctx, &mk, a.k_pages, s, box_rows);
@@ -769,7 +848,6 @@ int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs
         p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(v.n_slots) * v.slot_rows * D);
     }
     p.pieces = v.pieces;
-    p.cta_off = v.cta_off;
     p.pt_flat = v.pt_flat;
     p.mask = v.mask;
     p.err = ctx->d_err;

@@ -65,7 +65,7 @@ def reference(case, q, scale, exact_f32):
       plus the rounding of the exponent's argument, 2^-22 of the largest score; fp32 queries enter as two fp16 halves,
       2^-22 of |q| (each weight is off by that much, relatively, twice: it enters numerator and denominator)
     - a weight is rounded to fp16 before it meets V: 2^-11 (2^-22 when it is carried in two halves), and at least the
-      subnormal step, 2^-25 of a weight of 1, where the largest weight is between 1 and 2^8
+      subnormal step, 2^-25 of a weight of 1, where the largest weight is at least 1
     - the sum over S tokens is fp32: S * 2^-23 of the sum of magnitudes at most
     - the exponential is off by 2^-21; for fp16 results some are a cubic in x - rint(x), whose minimax error over [-1/2, 1/2] is
       7.48e-5 = 2^-13.70 of the value (its coefficients against 2^f on a grid of 4001 points). Like the scores' error it

@@ -19,20 +19,24 @@ extern "C" int tree_work(size_t batch, size_t H, size_t KVH, const uint32_t* pre
     mlcb::TreeWork w;
     mlcb::tree_work_list(s, t, max_ctas, &w);
     if (w.pieces.size() * 11 > out_words || w.splits.size() * 8 > split_words || w.row_split.size() > row_words) return 0;
-    for (size_t c = 0; c + 1 < w.cta_off.size(); ++c)
-        for (uint32_t i = w.cta_off[c]; i < w.cta_off[c + 1]; ++i) {
-            const mlcb::TreePiece& p = w.pieces[i];
-            const uint32_t v[11] = {static_cast<uint32_t>(c), p.kv_head, p.row_begin, p.n_rows, p.tile_begin, p.n_tiles, p.slot,
+    size_t n_out = 0;
+    for (uint32_t c = 0; c < w.n_cta; ++c)
+        for (uint32_t i = 0; i <= w.pieces[c].more; ++i, ++n_out) {
+            const size_t at = i ? w.pieces[c].next + i - 1 : c;
+            if (at >= w.pieces.size()) return 0;
+            const mlcb::TreePiece& p = w.pieces[at];
+            const uint32_t v[11] = {c, p.kv_head, p.row_begin, p.n_rows, p.tile_begin, p.n_tiles, p.slot,
                                     p.prefix, p.draft, p.token0, p.pt_off};
-            std::memcpy(out + 11 * i, v, sizeof(v));
+            std::memcpy(out + 11 * n_out, v, sizeof(v));
         }
+    if (n_out != w.pieces.size()) return 0;
     for (size_t i = 0; i < w.splits.size(); ++i) {
         const mlcb::TreeSplit& p = w.splits[i];
         const uint32_t v[8] = {p.kv_head, p.row_begin, p.n_rows, p.token0, p.first_slot, p.n_parts, p.first_row, p.slot_step};
         std::memcpy(splits + 8 * i, v, sizeof(v));
     }
     if (!w.row_split.empty()) std::memcpy(row_split, w.row_split.data(), w.row_split.size() * 4);
-    const uint32_t n[6] = {static_cast<uint32_t>(w.pieces.size()), static_cast<uint32_t>(w.cta_off.size() - 1),
+    const uint32_t n[6] = {static_cast<uint32_t>(w.pieces.size()), w.n_cta,
                            static_cast<uint32_t>(w.splits.size()), static_cast<uint32_t>(w.row_split.size()), w.n_slots, w.slot_rows};
     std::memcpy(counts, n, sizeof(n));
     return 1;

@@ -49,7 +49,7 @@ struct TreeWork {
     uint32_t n_cta = 0;
     std::vector<TreeSplit> splits;
     std::vector<uint32_t> row_split;  // split of every merged row
-    uint32_t n_slots = 0, slot_rows = 0;
+    uint32_t n_slots = 0, slot_rows = 0, max_parts = 0;
 };
 
 struct TreeView {   // device addresses inside one image
@@ -59,7 +59,7 @@ struct TreeView {   // device addresses inside one image
     const TreePiece* pieces = nullptr;
     const TreeSplit* splits = nullptr;
     const uint32_t* row_split = nullptr;
-    uint32_t n_cta = 0, n_slots = 0, slot_rows = 0, merge_rows = 0;
+    uint32_t n_cta = 0, n_slots = 0, slot_rows = 0, merge_rows = 0, max_parts = 0;
 };
 
 struct TreeArgs {

@@ -96,6 +96,7 @@ TreeView view_of(const uint8_t* dev, const TreeLayout& l, const TreeWork& w) {
     v.n_cta = w.n_cta;
     v.n_slots = w.n_slots;
     v.slot_rows = w.slot_rows;
+    v.max_parts = w.max_parts;
     v.merge_rows = static_cast<uint32_t>(w.row_split.size());
     return v;
 }

@@ -15,10 +15,14 @@ namespace mlcb {
 
 namespace {
 
-// Tiles a piece's fixed work (queries in, output or partial out) counts for.
-constexpr uint32_t kPieceCost = 2;
-// No cut leaves less than this: a short piece's partial costs more than the tiles it takes off another CTA.
-constexpr uint32_t kMinPiece = 4;
+// Tiles a piece's fixed work (queries in, output or partial out) counts for: 32 requests of 1 to 4095 tokens take 36.9 us
+// with 2, 35.8 with 4.
+constexpr uint32_t kPieceCost = 4;
+// No cut leaves less than this. One request of 1000 tokens, 8 drafted: 8.8 us with 2, 9.5 with 4, 11.6 with 8.
+constexpr uint32_t kMinPiece = 2;
+// Where every run has a CTA of its own and none is longer than this, nothing is cut: the second kernel costs more than
+// the tiles it saves. 16 requests of 500 tokens (8 tiles): 9.0 us whole, 11.6 cut; one of 1000 (16 tiles): 12.9 whole, 8.8 cut.
+constexpr uint32_t kWholeTiles = 9;
 constexpr uint32_t kLanes = 8;
 
 }  // namespace
@@ -27,7 +31,7 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
     out->pieces.clear();
     out->splits.clear();
     out->row_split.clear();
-    out->n_cta = out->n_slots = out->slot_rows = 0;
+    out->n_cta = out->n_slots = out->slot_rows = out->max_parts = 0;
     const uint32_t G = static_cast<uint32_t>(s.H / s.KVH);
     // Row tiles side by side, at most: beyond, they share a run through L2 in turns. One where there are too few CTAs for
     // a group of every width.
@@ -38,8 +42,8 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
         uint32_t rows, per;       // rows of all of them, rows of a full one
     };
     std::vector<Unit> units[kLanes + 1];
-    uint64_t total = 0;
-    uint32_t token0 = 0;
+    uint64_t total = 0, n_lanes = 0;
+    uint32_t token0 = 0, longest = 0;
     for (size_t r = 0; r < s.batch; ++r) {
         const uint32_t draft = t.draft[r];
         const uint64_t rows = static_cast<uint64_t>(draft) * G;
@@ -63,6 +67,8 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
                 u.piece.slot = kTreeNoSlot;
                 units[u.lanes].push_back(u);
                 total += static_cast<uint64_t>(tiles + kPieceCost) * u.lanes;
+                n_lanes += u.lanes;
+                longest = std::max(longest, tiles);
                 out->slot_rows = std::max(out->slot_rows, std::min(per, u.rows));
             }
         token0 += draft;
@@ -70,11 +76,12 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
     if (total == 0 || max_ctas == 0) return;
     std::vector<std::vector<TreePiece>> ctas;
     uint64_t quota = std::max<uint64_t>((total + max_ctas - 1) / max_ctas, kPieceCost + 1);
+    if (n_lanes <= max_ctas && longest <= kWholeTiles) quota = std::max<uint64_t>(quota, longest + kPieceCost);
     for (;; quota += quota / 32 + 1) {   // rounding at the cuts may need a CTA more than there are: try again with longer runs
         ctas.clear();
         out->splits.clear();
         out->row_split.clear();
-        out->n_slots = 0;
+        out->n_slots = out->max_parts = 0;
         std::vector<std::vector<TreePiece>> group;   // pieces of the CTAs of the current group
         uint64_t used = 0;
         auto close_group = [&] {
@@ -124,6 +131,7 @@ void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, 
                     out->splits.push_back(sp);
                 }
                 out->n_slots += n_parts * lanes;
+                out->max_parts = std::max(out->max_parts, n_parts);
             }
             if (used) close_group();
         }

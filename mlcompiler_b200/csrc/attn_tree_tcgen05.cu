@@ -42,7 +42,6 @@ constexpr uint32_t kTmemS = 128;
 constexpr uint32_t kTmemQ = 64;
 constexpr uint32_t kThreads = 224;
 constexpr uint32_t kStageBytes = 32 * 128;     // per softmax warp: 128 bytes of each of its rows, on the way in or out
-constexpr int kFmaPairs = 12;                  // of a tile's 32 pairs of columns: exponentials on the FMA pipe
 
 template <int D, bool EXACT>
 struct Config {
@@ -98,22 +97,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
     return *reinterpret_cast<float2*>(&d);
-}
-// 2^x for two x <= 127 on the FMA pipe: 2^n times a cubic for 2^f, n = rint(x), f = x - n in [-1/2, 1/2]. The coefficients are
-// the minimax ones for the relative error, 2^-13.7 (least squares reweighted until the error is level). x below -126 gives less
-// than 2^-125.
-__device__ __forceinline__ float2 ex2_fma(float2 x) {
-    const float magic = 12582912.0f;   // 1.5 * 2^23: adding it leaves rint(x) in the low bits
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
-    const float2 t = add2(x, make_float2(magic, magic));
-    const float2 n = add2(t, make_float2(-magic, -magic));
-    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
-    float2 p = fma2(f, make_float2(0.05517167f, 0.05517167f), make_float2(0.24261113f, 0.24261113f));
-    p = fma2(p, f, make_float2(0.69326097f, 0.69326097f));
-    p = fma2(p, f, make_float2(0.99992806f, 0.99992806f));
-    return make_float2(__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23)));
 }
 __device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -573,8 +556,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                         for (int i = 0; i < 32; ++i) {
                             const float2 raw = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
                             float2 x = fma2(raw, scale2, neg_m2);
-                            if (!EXACT && kFmaPairs * i % 32 < kFmaPairs) x = ex2_fma(x);
-                            else x = make_float2(ex2(x.x), ex2(x.y));
+                            x = make_float2(ex2(x.x), ex2(x.y));
                             ps[i & 1] = add2(ps[i & 1], x);
                             const __half2 h = __float22half2_rn(x);
                             hi[i] = *reinterpret_cast<const uint32_t*>(&h);
@@ -664,7 +646,6 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
             if (!ok) break;
             tc::fence_after();
-            if (l_sum < 1e-30f) l_sum = 0.f;   // a row that saw nothing: what ex2_fma leaves of -inf
             if (busy) {
                 const bool mine = row < done.n_rows;
                 const bool whole = done.slot == kTreeNoSlot;
@@ -721,76 +702,65 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     if (warp == 4) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
-// O of the rows whose unit was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. WARPS warps per row
-// take the parts round-robin; a lane holds D / 32 columns.
+// O of the rows whose run was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. WARPS warps per row
+// take the parts round-robin, eight in flight at a time. The tables are read before the wait for the kernel in front.
 template <int D, int WARPS, typename OT>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
                                                          const TreeSplit* __restrict__ splits, const uint32_t* __restrict__ row_split,
                                                          OT* __restrict__ o, uint32_t rows, uint32_t slot_rows, uint32_t H, uint32_t G) {
-    constexpr int V = D / 32;
-    constexpr int kRowsPerCta = 4 / WARPS;
-    __shared__ float s_o[WARPS > 1 ? WARPS : 1][D];
-    __shared__ float2 s_ml[4];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    constexpr int kLanes = D / 4;               // lanes a part's row takes, four columns each
+    constexpr int kAtOnce = 32 / kLanes;        // parts a warp reads with one instruction
+    constexpr int kStride = WARPS * kAtOnce;
+    __shared__ float4 s_o[WARPS > 1 ? WARPS : 1][kLanes];
+    __shared__ float s_l[4];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t row = blockIdx.x * kRowsPerCta + warp / WARPS, sub = warp % WARPS;
+    const uint32_t row = blockIdx.x * (4 / WARPS) + warp / WARPS, sub = warp % WARPS;
     if (row >= rows) return;   // with WARPS > 1 a CTA has one row: all or none leave
     const TreeSplit sp = splits[row_split[row]];
     const uint32_t r = row - sp.first_row;
     auto index = [&](uint32_t k) { return static_cast<size_t>(sp.first_slot + k * sp.slot_step) * slot_rows + r; };
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     float top = -INFINITY;
-    for (uint32_t k = sub * 32 + lane; k < sp.n_parts; k += WARPS * 32) top = fmaxf(top, __ldcg(&part_ml[index(k)]).x);
+    for (uint32_t k = lane; k < sp.n_parts; k += 32) top = fmaxf(top, __ldcg(&part_ml[index(k)]).x);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if constexpr (WARPS > 1) {
-        if (lane == 0) s_ml[warp].x = top;
-        __syncthreads();
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, s_ml[w].x);
-        __syncthreads();
-    }
-    float acc[V] = {}, l = 0.f;
-#pragma unroll 4
-    for (uint32_t k = sub; k < sp.n_parts; k += WARPS) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 8
+    for (uint32_t k = sub * kAtOnce + lane / kLanes; k < sp.n_parts; k += kStride) {
         const float2 ml = __ldcg(&part_ml[index(k)]);
-        const float* src = part_o + index(k) * D + lane * V;
-        float v[V];
-        if constexpr (V == 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-            v[0] = x.x; v[1] = x.y;
-        }
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_o + index(k) * D) + lane % kLanes);
         // a part that saw nothing has m = -inf, l = 0 and o = 0
         const float w = ml.x == -INFINITY ? 1.0f : ex2(ml.x - top);
         l += ml.y * w;
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += v[i] * w;
+        acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+    }
+    if constexpr (kAtOnce == 2) {
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
+        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
+        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
+        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
     }
     if constexpr (WARPS > 1) {
-        if (lane == 0) s_ml[warp].y = l;
-#pragma unroll
-        for (int i = 0; i < V; ++i) s_o[sub][lane * V + i] = acc[i];
+        if (lane == 0) s_l[warp] = l;
+        if (lane < kLanes) s_o[sub][lane] = acc;
         __syncthreads();
         if (sub) return;
         l = 0.f;
-        for (int w = 0; w < WARPS; ++w) l += s_ml[w].y;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            acc[i] = 0.f;
-            for (int w = 0; w < WARPS; ++w) acc[i] += s_o[w][lane * V + i];
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 v = s_o[w][lane % kLanes];
+            l += s_l[w];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
         }
     }
+    if (lane >= kLanes) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const uint32_t rr = sp.row_begin + r;
-    OT* dst = o + (static_cast<size_t>(sp.token0 + rr / G) * H + sp.kv_head * G + rr % G) * D + lane * V;
-    if constexpr (sizeof(OT) == 4) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) dst[i] = acc[i] * inv;
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = pack(acc[i] * inv, acc[i + 1] * inv);
-    }
+    OT* dst = o + (static_cast<size_t>(sp.token0 + rr / G) * H + sp.kv_head * G + rr % G) * D + lane * 4;
+    if constexpr (sizeof(OT) == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack(acc.x * inv, acc.y * inv), pack(acc.z * inv, acc.w * inv));
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -816,8 +786,8 @@ int pool_map(mlc_ctx* ctx, CUtensorMap* out, const void* pool, const TreeShape& 
 
 template <int D, typename OT>
 cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const float* part_o, const float2* part_ml, void* o) {
-    // few rows: four warps share one, the parts are read four at a time
-    const bool wide = v.merge_rows <= 4u * static_cast<uint32_t>(ctx->sm_count) * 4u;
+    // many parts a row: four warps share it
+    const bool wide = v.max_parts > 8;
     auto kernel = wide ? tree_merge_kernel<D, 4, OT> : tree_merge_kernel<D, 1, OT>;
     const dim3 grid(wide ? v.merge_rows : (v.merge_rows + 3) / 4);
     return launch_dependent(ctx, kernel, grid, 128, 0, part_o, part_ml, v.splits, v.row_split, static_cast<OT*>(o), v.merge_rows,

@@ -93,11 +93,11 @@ _PROTOTYPES = {
     "mlc_tree_plan_update": (_i, [_vp, _vp, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz]),
     "mlc_tree_plan_destroy": (None, [_vp, _vp]),
     "mlc_encode_paged_tree_attention_planned": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _f, _i, _i]),
-    "mlc_run_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _u32p, _sz, _sz, _sz, _sz, _sz, _sz]),
-    "mlc_encode_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _u32p, _sz, _sz, _sz, _sz, _sz, _sz]),
-    "mlc_run_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz, _sz,
+    "mlc_run_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "mlc_encode_copy_kv_pages": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz]),
+    "mlc_run_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz,
                                      _sz, _sz]),
-    "mlc_encode_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _u32p, _sz, _u32p, _u32p, _u32p, _u32p, _sz, _sz, _sz,
+    "mlc_encode_compact_kv_rows": (_i, [_vp, C.POINTER(_vp), _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _sz, _sz,
                                         _sz, _sz, _sz]),
     "mlc_compute_rotary_coefficients": (_i, [_sz, _sz, _f, _f, C.POINTER(C.c_float), C.POINTER(C.c_float)]),
     "mlc_exchange_create": (_i, [_vp, _i, _i, _sz, _sz, C.POINTER(_vp)]),
@@ -165,6 +165,13 @@ def _ptr(x) -> int:
     if hasattr(x, "data_ptr"):
         return int(x.data_ptr())
     raise TypeError(f"not a device buffer: {type(x)}")
+
+
+def _u32_at(a):
+    """Like _u32, with the address as an integer: what the calls of a step's hot path pass."""
+    if type(a) is not np.ndarray or a.dtype != np.uint32 or not a.flags.c_contiguous:
+        a = np.ascontiguousarray(np.asarray(a, dtype=np.uint32))
+    return a, a.ctypes.data
 
 
 def _u32(a):
@@ -640,8 +647,8 @@ class Executor:
 
     def _copyPages(self, fn, pools, src_page_ids, dst_page_ids, page_size_tokens, n_kv_heads, head_dim, dtype_bytes,
                    capacity_pages) -> bool:
-        src, psrc = _u32(src_page_ids)
-        dst, pdst = _u32(dst_page_ids)
+        src, psrc = _u32_at(src_page_ids)
+        dst, pdst = _u32_at(dst_page_ids)
         if src.size != dst.size:
             return self.status(1)
         return self.status(fn(self._h, pools, len(pools), psrc, pdst, src.size, page_size_tokens, n_kv_heads, head_dim,
@@ -660,11 +667,11 @@ class Executor:
 
     def _compactRows(self, fn, pools, page_tables_flat, page_table_offsets, start_positions, kept_rows, kept_offsets, batch,
                      page_size_tokens, n_kv_heads, head_dim, dtype_bytes, capacity_pages) -> bool:
-        flat, pflat = _u32(page_tables_flat)
-        off, poff = _u32(page_table_offsets)
-        start, pstart = _u32(start_positions)
-        kept, pkept = _u32(kept_rows)
-        koff, pkoff = _u32(kept_offsets)
+        flat, pflat = _u32_at(page_tables_flat)
+        off, poff = _u32_at(page_table_offsets)
+        start, pstart = _u32_at(start_positions)
+        kept, pkept = _u32_at(kept_rows)
+        koff, pkoff = _u32_at(kept_offsets)
         if off.size != batch + 1 or start.size != batch or koff.size != batch + 1 or kept.size < int(koff[-1]):
             return self.status(1)
         return self.status(fn(self._h, pools, len(pools), pflat, flat.size, poff, pstart, pkept, pkoff, batch,

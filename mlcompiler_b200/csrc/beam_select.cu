@@ -6,14 +6,18 @@
 // (compiler/runtime/scheduler.cpp:101-118); this stands beside the device argmax.
 //
 // What bounds it: every logit is read once, so the memory's read bandwidth for large calls; a launch and the two chained
-// steps for small ones. One pass over the logits does both jobs: a CTA holds a chunk of a row in registers, takes its
-// maximum, its sum of exponentials and its n_select largest values, and the last CTA of a group to finish joins the chunks.
-// Inside a row the order by score is the order by logit, so a chunk needs no logarithm. The values of a chunk are
-// found with a threshold: the n_select-th largest of 64 maxima over disjoint parts of the chunk has at least n_select
-// values at or above it, and on real logits few more. The cross-beam comparison needs the differences of nearly
-// equal sums: sums over 32 values are taken in fp32, what joins them and the scores in fp64.
+// steps for small ones. One pass over the logits does both jobs: a warp walks a segment of a row, 512 logits a step with
+// the next step's in flight, and keeps a running maximum, a running sum of exponentials and the n_select largest logits
+// so far; the last CTA of a group to finish joins the segments. Inside a row the order by score is the order by logit, so a
+// segment needs no logarithm. The largest logits are kept as a list in shared memory with a threshold, the n_select-th
+// largest at the last clean-up: on real logits few pass it after the first step, and a step in which none does costs one
+// vote. Warps work on their own: 512 rows of 128000, a quarter of them finished, take 64 us (the read of all of them 40); with a CTA
+// per 8192 logits and its five barriers it was 180.
+// The comparison between beams needs the differences of nearly equal sums: a lane's sum over a step is taken in fp32,
+// what joins the segments and the scores in fp64.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cstring>
 
 #include "op_util.hpp"
@@ -22,24 +26,28 @@ namespace mlcb {
 
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kParts = 64;        // maxima the threshold is taken from: one per four threads
-constexpr uint32_t kMaxSelect = 64;    // = kParts: the threshold needs that many
+constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
+constexpr uint32_t kCtasPerSm = 3;     // four would leave 64 registers a thread: 76 us instead of 63 for 512 rows of 128000
+constexpr uint32_t kStep = 512;        // logits a warp takes at a time: four float4 a lane
+constexpr uint32_t kParts = 64;        // maxima a threshold is taken from
+constexpr uint32_t kMaxSelect = 64;    // = kParts: a threshold needs that many
 constexpr uint32_t kMaxBeams = 64;
-constexpr uint32_t kListCap = 512;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kListCap = 128;     // of a warp's list
+constexpr uint32_t kFoundCap = 1024;   // of the joining CTA's
+constexpr uint32_t kMaxLists = 512;    // segments of a group's rows that one CTA should join
+constexpr float kLog2e = 1.4426950408889634f, kLowest = -3.402823466e38f;
 
 struct BeamParams {
     const float* logits;
     const float* cum;
     const uint8_t* finished;   // may be null
-    uint64_t* keys;            // [rows * chunks][n_select]
-    float2* sums;              // [rows * chunks] (maximum, sum of exponentials relative to it)
+    uint64_t* keys;            // [rows * segments][n_select]
+    float2* sums;              // [rows * segments] (maximum, sum of exponentials relative to it)
     uint32_t* counters;        // [groups], zero between launches
     float* out_scores;
     uint32_t* out_parents;
     uint32_t* out_tokens;
-    uint32_t rows, beams, vocab, group_rows, chunks_per_part, chunks, chunk_len, n_select, pad;
+    uint32_t rows, beams, vocab, group_rows, per_block, segments, segment_len, ctas_per_group, n_select, pad;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -49,6 +57,23 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // exp(a - b) for a <= b; b > -inf
 __device__ __forceinline__ float exp_diff(float a, float b) { return ex2((a - b) * kLog2e); }
+
+// Two fp32 operations in one instruction, on register pairs.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(*reinterpret_cast<uint64_t*>(&a)), "l"(*reinterpret_cast<uint64_t*>(&b)));
+    return *reinterpret_cast<float2*>(&d);
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // passes over NaN
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 
 // Larger key = larger value, then lower token; 0 is below every key.
 __device__ __forceinline__ uint64_t make_key(float x, uint32_t token) {
@@ -62,24 +87,27 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_token(uint64_t key) { return 0xFFFFFFFFu - static_cast<uint32_t>(key); }
 
-// The k-th largest of 64 values in shared memory, computed by one warp (every lane gets it).
+// The k-th largest of 64 values in shared memory, by one warp (every lane gets it): the smallest value that fewer than k of
+// them exceed.
 template <typename T>
-__device__ __forceinline__ T kth_of_64(const T* v, uint32_t k, uint32_t lane, T lowest) {
+__device__ __forceinline__ T kth_of_64(const T* v, uint32_t k, uint32_t lane) {
     const T a = v[lane], b = v[lane + 32];
-    uint32_t above_a = 0, above_b = 0, with_a = 0, with_b = 0;
-#pragma unroll 8
+    uint32_t above_a = 0, above_b = 0;
+#pragma unroll 16
     for (uint32_t j = 0; j < 64; ++j) {
         const T x = v[j];
         above_a += x > a;
         above_b += x > b;
-        with_a += x >= a;
-        with_b += x >= b;
     }
-    const bool is_a = above_a < k && k <= with_a, is_b = above_b < k && k <= with_b;
-    const uint32_t va = __ballot_sync(0xffffffffu, is_a), vb = __ballot_sync(0xffffffffu, is_b);
-    if (va) return __shfl_sync(0xffffffffu, a, __ffs(va) - 1);
-    if (vb) return __shfl_sync(0xffffffffu, b, __ffs(vb) - 1);
-    return lowest;
+    T kth = static_cast<T>(INFINITY);
+    if (above_a < k) kth = a;
+    if (above_b < k && b < kth) kth = b;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const T x = __shfl_xor_sync(0xffffffffu, kth, o);
+        if (x < kth) kth = x;
+    }
+    return kth;
 }
 
 struct Candidate {
@@ -92,77 +120,87 @@ __device__ __forceinline__ bool better(const Candidate& a, const Candidate& b) {
 }
 
 struct Shared {
-    uint64_t list[kListCap];
-    Candidate found[kListCap];
-    double part_d[kParts];
+    uint32_t listed[kWarps];
+    union {
+        uint64_t list[kWarps][kListCap];
+        Candidate found[kFoundCap];
+    };
+    float tops[kThreads];
     double lse[kMaxBeams];
-    float part[kParts];
-    float warp_m[8], warp_s[8];
-    uint64_t warp_key[8];
-    Candidate warp_best[8];
-    float threshold;
-    double threshold_d;
+    float part[kWarps][kParts];
+    Candidate warp_best[kWarps];
     uint32_t count, last;
 };
 
-// Joins the chunks of one group: run by the CTA that finished last.
+// Joins the segments of one group: run by the CTA that finished last.
 __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_t group) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row0 = group * p.beams;
-    for (uint32_t b = warp; b < p.beams; b += kThreads / 32) {
+    const uint32_t row0 = group * p.beams, lists = p.beams * p.segments;
+    // the head of this thread's first list is on its way while the sums are joined
+    const uint64_t head_key = tid < lists ? __ldcg(&p.keys[(static_cast<size_t>(row0) * p.segments + tid) * p.n_select]) : 0;
+    for (uint32_t b = warp; b < p.beams; b += kWarps) {
+        const float2* sums = p.sums + static_cast<size_t>(row0 + b) * p.segments;
         float m = -INFINITY;
-        for (uint32_t c = lane; c < p.chunks; c += 32) m = fmaxf(m, __ldcg(&p.sums[static_cast<size_t>(row0 + b) * p.chunks + c].x));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         double s = 0.0;
-        for (uint32_t c = lane; c < p.chunks; c += 32) {
-            const float2 ms = __ldcg(&p.sums[static_cast<size_t>(row0 + b) * p.chunks + c]);
-            if (ms.x > -INFINITY || ms.y != 0.0f) s += static_cast<double>(ms.y) * exp(static_cast<double>(ms.x) - static_cast<double>(m));
+        for (uint32_t i = lane; i < p.segments; i += 32) {   // a segment of -inf alone has the sum 0
+            const float2 v = __ldcg(sums + i);
+            const float both = fmaxf(m, v.x);
+            if (both > -INFINITY) s = s * static_cast<double>(exp_diff(m, both)) + static_cast<double>(v.y) * static_cast<double>(exp_diff(v.x, both));
+            m = both;
         }
+        float all = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+        if (m > -INFINITY) s *= static_cast<double>(exp_diff(m, all));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         // (a row of -inf alone has no candidates that would use it; one with +inf gives NaN, and so no candidates)
-        if (lane == 0) sh.lse[b] = static_cast<double>(m) + log(s);
+        if (lane == 0) sh.lse[b] = static_cast<double>(all) + log(s);
     }
     if (tid == 0) sh.count = 0;
     __syncthreads();
 
-    const uint32_t per_row = p.chunks * p.n_select, total = p.beams * per_row;
-    // candidate i of the group: a chunk's list entry; behind them one per beam for finished beams
-    auto candidate = [&](uint32_t i, Candidate& c) {
-        if (i >= total) {
-            const uint32_t b = i - total;
-            if (!p.finished || !p.finished[row0 + b]) return false;
-            c = {static_cast<double>(p.cum[row0 + b]), b, p.pad};
+    // Candidate c of list i: of a segment, largest first, or - behind the segments' lists - the only one of a finished beam.
+    auto candidate = [&](uint32_t i, uint32_t c, Candidate& got) {
+        if (i >= lists) {
+            const uint32_t b = i - lists;
+            if (c || !p.finished || !p.finished[row0 + b]) return false;
+            got = {static_cast<double>(p.cum[row0 + b]), b, p.pad};
         } else {
-            const uint32_t b = i / per_row;
-            if (p.finished && p.finished[row0 + b]) return false;
-            const uint64_t key = __ldcg(&p.keys[static_cast<size_t>(row0) * per_row + i]);
+            const uint32_t b = i / p.segments;
+            if (c >= p.n_select || (p.finished && p.finished[row0 + b])) return false;
+            const uint64_t key = i == tid && c == 0 ? head_key : __ldcg(&p.keys[(static_cast<size_t>(row0) * p.segments + i) * p.n_select + c]);
             if (key == 0) return false;
-            c = {static_cast<double>(p.cum[row0 + b]) + (static_cast<double>(key_value(key)) - sh.lse[b]), b, key_token(key)};
+            got = {static_cast<double>(p.cum[row0 + b]) + (static_cast<double>(key_value(key)) - sh.lse[b]), b, key_token(key)};
         }
-        return c.score > -INFINITY;   // not for NaN either
+        return got.score > -INFINITY;   // not for NaN either
     };
-    double top = -INFINITY;
-    for (uint32_t i = tid; i < total + p.beams; i += kThreads) {
+    // The n_select-th largest of 64 maxima over parts of the lists' first entries: at least that many candidates reach it. With
+    // 64 lists or more a head each is enough, with fewer each gives several.
+    const uint32_t deep = min(p.n_select, (2 * kParts - 1) / lists + 1);
+    float top = -INFINITY;   // rounded down: no more than a few candidates too many pass
+    for (uint32_t i = tid; i < lists * deep + p.beams; i += kThreads) {
+        const uint32_t d = i / lists;
         Candidate c;
-        if (candidate(i, c)) top = fmax(top, c.score);
+        if (d < deep ? candidate(i - d * lists, d, c) : candidate(i - lists * deep + lists, 0, c)) top = fmaxf(top, __double2float_rd(c.score));
     }
-    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmax(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if ((tid & 3) == 0) sh.part_d[tid >> 2] = top;
+    sh.tops[tid] = top;
     __syncthreads();
     if (warp == 0) {
-        const double t = kth_of_64(sh.part_d, p.n_select, lane, static_cast<double>(-INFINITY));
-        if (lane == 0) sh.threshold_d = t;
+        for (uint32_t i = lane; i < kParts; i += 32)
+            sh.tops[i] = fmaxf(fmaxf(sh.tops[i], sh.tops[i + 64]), fmaxf(sh.tops[i + 128], sh.tops[i + 192]));
+        __syncwarp();
+        const float t = kth_of_64(sh.tops, p.n_select, lane);
+        __syncwarp();
+        if (lane == 0) sh.tops[0] = t;
     }
     __syncthreads();
-    const double threshold = sh.threshold_d;
-    for (uint32_t i = tid; i < total + p.beams; i += kThreads) {
+    const float threshold = sh.tops[0];
+    for (uint32_t i = tid; i < lists + p.beams; i += kThreads) {
         Candidate c;
-        if (candidate(i, c) && c.score >= threshold) {
+        for (uint32_t j = 0; candidate(i, j, c) && c.score >= threshold; ++j) {
             const uint32_t at = atomicAdd(&sh.count, 1u);
-            if (at < kListCap) sh.found[at] = c;
+            if (at < kFoundCap) sh.found[at] = c;
         }
     }
     __syncthreads();
@@ -174,7 +212,7 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
         p.out_tokens[out + at] = c.token;
     };
     uint32_t have = n;
-    if (n <= kListCap) {
+    if (n <= kFoundCap) {
         for (uint32_t i = tid; i < n; i += kThreads) {
             const Candidate mine = sh.found[i];
             uint32_t rank = 0;
@@ -187,9 +225,13 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
         bool first = true;
         for (have = 0; have < p.n_select; ++have) {
             Candidate best{-INFINITY, 0xFFFFFFFFu, 0xFFFFFFFFu};
-            for (uint32_t i = tid; i < total + p.beams; i += kThreads) {
+            for (uint32_t i = tid; i < lists + p.beams; i += kThreads) {
                 Candidate c;
-                if (candidate(i, c) && (first || better(last, c)) && better(c, best)) best = c;
+                for (uint32_t j = 0; candidate(i, j, c); ++j) {   // the first of a list that is not taken yet is its best
+                    if (!first && !better(last, c)) continue;
+                    if (better(c, best)) best = c;
+                    break;
+                }
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) {
@@ -200,7 +242,7 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
             if (lane == 0) sh.warp_best[warp] = best;
             __syncthreads();
             best = sh.warp_best[0];
-            for (uint32_t w = 1; w < kThreads / 32; ++w)
+            for (uint32_t w = 1; w < kWarps; ++w)
                 if (better(sh.warp_best[w], best)) best = sh.warp_best[w];
             __syncthreads();
             if (!(best.score > -INFINITY)) break;
@@ -212,130 +254,209 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
     for (uint32_t i = have + tid; i < p.n_select; i += kThreads) write(i, {-INFINITY, 0xFFFFFFFFu, 0xFFFFFFFFu});
 }
 
-// NV: float4 vectors of a chunk that a thread holds.
-template <int NV>
-__global__ void __launch_bounds__(kThreads) beam_select_kernel(const __grid_constant__ BeamParams p) {
+// Keeps the `keep` largest of a warp's n <= 32 * PER listed keys, largest first; returns how many there are.
+template <uint32_t PER>
+__device__ __forceinline__ uint32_t shorten_to(uint64_t* list, uint32_t n, uint32_t keep, uint32_t lane) {
+    uint64_t mine[PER];
+    uint32_t rank[PER];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i) {
+        mine[i] = lane + 32 * i < n ? list[lane + 32 * i] : 0;
+        rank[i] = 0;
+    }
+#pragma unroll 4
+    for (uint32_t j = 0; j < n; ++j) {
+        const uint64_t k = list[j];
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) rank[i] += k > mine[i];
+    }
+    __syncwarp();
+#pragma unroll
+    for (uint32_t i = 0; i < PER; ++i)
+        if (mine[i] && rank[i] < keep) list[rank[i]] = mine[i];
+    __syncwarp();
+    return min(n, keep);
+}
+__device__ __noinline__ uint32_t shorten(uint64_t* list, uint32_t n, uint32_t keep, uint32_t lane) {
+    if (n <= 32) return shorten_to<1>(list, n, keep, lane);
+    if (n <= 64) return shorten_to<2>(list, n, keep, lane);
+    return shorten_to<kListCap / 32>(list, n, keep, lane);
+}
+
+// Sum of the exponentials of 16 logits on top of s, relative to the running maximum m; `quarter` receives the largest of every
+// four of them.
+__device__ __forceinline__ float add_step(const float (&x)[16], float& m, float& s, float (&quarter)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) quarter[j] = fmaxf(max3(x[4 * j], x[4 * j + 1], x[4 * j + 2]), x[4 * j + 3]);   // passes over NaN
+    const float top = fmaxf(max3(quarter[0], quarter[1], quarter[2]), quarter[3]);
+    const float both = fmaxf(m, top), ref = both == -INFINITY ? 0.f : both;
+    const float2 minus = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
+    float2 t[2] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {   // the difference first: its rounding is relative to it, not to the maximum
+        const float2 d = mul2(add2(make_float2(x[2 * i], x[2 * i + 1]), minus), log2e);
+        t[i & 1] = add2(t[i & 1], make_float2(ex2(d.x), ex2(d.y)));
+    }
+    t[0] = add2(t[0], t[1]);
+    s = s * exp_diff(m, ref) + (t[0].x + t[0].y);
+    m = both;
+    return top;
+}
+
+// One segment of a row, by one warp.
+__device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uint32_t* listed, float* part, uint32_t row, uint32_t seg, uint32_t lane) {
+    const uint32_t block = seg / p.per_block, begin = (seg - block * p.per_block) * p.segment_len;
+    const uint32_t block_rows = min(p.group_rows, p.vocab - block * p.group_rows);
+    const int len = begin < block_rows ? static_cast<int>(min(p.segment_len, block_rows - begin)) : 0;   // the last block may be short
+    const float* x0 = p.logits + static_cast<size_t>(p.rows) * block * p.group_rows + static_cast<size_t>(row) * block_rows + begin;
+    // The body is whole float4s; up to three logits in front of it and behind it are taken first, a lane each.
+    const int head = min(static_cast<int>((16u - (static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x0)) & 15u)) & 15u) / 4, len);
+    const int vecs = (len - head) / 4, edges = head + ((len - head) & 3);
+    const int steps = (vecs + static_cast<int>(kStep / 4) - 1) / static_cast<int>(kStep / 4);
+    const uint32_t token0 = block * p.group_rows + begin;
+    const float4* body = reinterpret_cast<const float4*>(x0 + head);
+    // Loads are the same in every step: a lane whose vector lies behind the body reads the last one again, and drops it.
+    auto load = [&](int step, float (&x)[16]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float4 v = __ldcs(body + min(step * static_cast<int>(kStep / 4) + static_cast<int>(lane) + 32 * j, vecs - 1));
+            x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+        }
+    };
+    auto drop_behind = [&](int step, float (&x)[16]) {
+        if ((step + 1) * static_cast<int>(kStep / 4) <= vecs) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (step * static_cast<int>(kStep / 4) + static_cast<int>(lane) + 32 * j >= vecs)
+                x[4 * j] = x[4 * j + 1] = x[4 * j + 2] = x[4 * j + 3] = -INFINITY;
+    };
+    float m = -INFINITY, s = 0.f, threshold = kLowest;   // (at least the lowest number, so that -inf never passes)
+    uint64_t lowest = 0;    // once n_select keys are listed: the n_select-th
+    uint32_t n = 0;
+    auto clean_up = [&] {
+        n = shorten(list, n, p.n_select, lane);
+        lowest = list[p.n_select - 1];
+        threshold = fmaxf(threshold, key_value(lowest));
+        __syncwarp();
+    };
+    float next[16];
+    if (steps) load(0, next);
+    const int edge_at = static_cast<int>(lane) < head ? static_cast<int>(lane) : 4 * vecs + static_cast<int>(lane);
+    const float edge = static_cast<int>(lane) < edges ? x0[edge_at] : -INFINITY;
+    if (edges) {
+        if (edge > -INFINITY) {
+            m = edge;
+            s = exp_diff(edge, edge);   // 1, or NaN of +inf
+        }
+        const uint32_t in = __ballot_sync(0xffffffffu, edge > -INFINITY);
+        if ((in >> lane) & 1u) list[__popc(in & ((1u << lane) - 1u))] = make_key(edge + 0.0f, token0 + edge_at);
+        n = __popc(in);
+        __syncwarp();
+    }
+#pragma unroll 1
+    for (int step = 0; step < steps; ++step) {
+        float x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = next[i];
+        if (step + 1 < steps) load(step + 1, next);
+        drop_behind(step, x);
+        float quarter[4];
+        const float top = add_step(x, m, s, quarter);
+        if (step == 0) {
+            // The n_select-th largest of 64 maxima over parts of the step has that many logits at or above it.
+            float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                a = max3(a, x[i], x[i + 1]);
+                b = max3(b, x[8 + i], x[9 + i]);
+            }
+            part[lane] = a;
+            part[lane + 32] = b;
+            __syncwarp();
+            threshold = fmaxf(kLowest, kth_of_64(part, p.n_select, lane));
+        }
+        if (!__any_sync(0xffffffffu, top >= threshold)) continue;
+        const uint32_t token = token0 + head + step * kStep + 4 * lane;
+        auto key_of = [&](int i) { return make_key(x[i] + 0.0f, token + 128 * (i >> 2) + (i & 3)); };   // -0 and 0 are one value
+        if (lane == 0) *listed = n;
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (quarter[j] >= threshold) {
+#pragma unroll
+                for (int i = 4 * j; i < 4 * j + 4; ++i)
+                    if (x[i] >= threshold) {
+                        const uint32_t at = atomicAdd(listed, 1u);
+                        if (at < kListCap) list[at] = key_of(i);
+                    }
+            }
+        __syncwarp();
+        const uint32_t now = *listed;
+        __syncwarp();
+        if (now <= kListCap) {
+            n = now;
+        } else {
+            // more than there is room for: once more, 32 at a time, with clean-ups in between
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (!__any_sync(0xffffffffu, x[i] >= threshold)) continue;
+                if (n + 32 > kListCap) clean_up();
+                const uint64_t key = key_of(i);
+                const uint32_t in = __ballot_sync(0xffffffffu, x[i] >= threshold && key > lowest);
+                if ((in >> lane) & 1u) list[n + __popc(in & ((1u << lane) - 1u))] = key;
+                n += __popc(in);
+                __syncwarp();
+            }
+        }
+        if (n >= 2 * p.n_select && n > 32) clean_up();   // worth a higher threshold
+    }
+    if (__any_sync(0xffffffffu, !(s == s))) {   // NaN among the logits counts as -inf (a sum that +inf spoils stays NaN)
+        m = edge > -INFINITY ? edge : -INFINITY;
+        s = edge > -INFINITY ? exp_diff(edge, edge) : 0.f;
+#pragma unroll 1
+        for (int step = 0; step < steps; ++step) {
+            float x[16];
+            load(step, x);
+            drop_behind(step, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (!(x[i] == x[i])) x[i] = -INFINITY;
+            float quarter[4];
+            add_step(x, m, s, quarter);
+        }
+    }
+    float top = m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    s = m > -INFINITY ? s * exp_diff(m, top) : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    n = shorten(list, n, p.n_select, lane);
+    const size_t unit = static_cast<size_t>(row) * p.segments + seg;
+    if (lane == 0) p.sums[unit] = make_float2(top, s);
+    for (uint32_t i = lane; i < p.n_select; i += 32) p.keys[unit * p.n_select + i] = i < n ? list[i] : 0;
+}
+
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) beam_select_kernel(const __grid_constant__ BeamParams p) {
     __shared__ Shared sh;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t row = blockIdx.x / p.chunks, chunk = blockIdx.x - row * p.chunks;
-    const uint32_t group = row / p.beams;
-    if (!p.finished || !p.finished[row]) {
-        const uint32_t part = chunk / p.chunks_per_part, begin = (chunk - part * p.chunks_per_part) * p.chunk_len;
-        const uint32_t part_rows = min(p.group_rows, p.vocab - part * p.group_rows);
-        const uint32_t len = begin < part_rows ? min(p.chunk_len, part_rows - begin) : 0u;   // the last part may be short
-        const uint32_t token0 = part * p.group_rows + begin;
-        const float* x0 = p.logits + static_cast<size_t>(p.rows) * part * p.group_rows + static_cast<size_t>(row) * part_rows + begin;
-        const uint32_t lead = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(x0) >> 2) & 3u;   // floats behind a 16-byte boundary
-        float x[NV][4];
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int at = static_cast<int>(4 * (tid + kThreads * j)) - static_cast<int>(lead);
-            if (at >= 0 && at + 4 <= static_cast<int>(len)) {
-                const float4 v = __ldcs(reinterpret_cast<const float4*>(x0 + at));
-                x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[j][e] = at + e >= 0 && at + e < static_cast<int>(len) ? x0[at + e] : -INFINITY;
-            }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[j][e] += 0.0f;                                     // -0 and 0 are one value
-                if (!(x[j][e] == x[j][e])) x[j][e] = -INFINITY;      // NaN
-                top = fmaxf(top, x[j][e]);
-            }
-        float s = 0.0f;
-        if (top > -INFINITY) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j)
-                s += (exp_diff(x[j][0], top) + exp_diff(x[j][1], top)) + (exp_diff(x[j][2], top) + exp_diff(x[j][3], top));
-        }
-        float quad = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        quad = fmaxf(quad, __shfl_xor_sync(0xffffffffu, quad, 2));
-        if ((tid & 3) == 0) sh.part[tid >> 2] = quad;
-        float m = quad;
-#pragma unroll
-        for (int o = 16; o > 2; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        s = top > -INFINITY ? s * exp_diff(top, m) : 0.0f;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) { sh.warp_m[warp] = m; sh.warp_s[warp] = s; }
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        if (warp == 0) {
-            const float t = kth_of_64(sh.part, p.n_select, lane, -INFINITY);
-            if (lane == 0) sh.threshold = t;
-        } else if (tid == 32) {
-            float all = -INFINITY;
-            for (int w = 0; w < 8; ++w) all = fmaxf(all, sh.warp_m[w]);
-            double sum = 0.0;
-            for (int w = 0; w < 8; ++w)
-                if (sh.warp_m[w] > -INFINITY) sum += static_cast<double>(sh.warp_s[w]) * static_cast<double>(exp_diff(sh.warp_m[w], all));
-            p.sums[blockIdx.x] = make_float2(all, static_cast<float>(sum));
-        }
-        __syncthreads();
-        const float threshold = sh.threshold;
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (x[j][e] >= threshold && x[j][e] > -INFINITY) {
-                    const uint32_t at = atomicAdd(&sh.count, 1u);
-                    if (at < kListCap) sh.list[at] = make_key(x[j][e], token0 + 4 * (tid + kThreads * j) + e - lead);
-                }
-        __syncthreads();
-        uint64_t* keys = p.keys + static_cast<size_t>(blockIdx.x) * p.n_select;
-        const uint32_t n = sh.count;
-        uint32_t have = n;
-        if (n <= kListCap) {
-            for (uint32_t i = tid; i < n; i += kThreads) {
-                const uint64_t mine = sh.list[i];
-                uint32_t rank = 0;
-                for (uint32_t j = 0; j < n; ++j) rank += sh.list[j] > mine;
-                if (rank < p.n_select) keys[rank] = mine;
-            }
-        } else {
-            // many equal values at the threshold: take the best key, then the best below it, and so on
-            uint64_t last = ~0ull;
-            for (have = 0; have < p.n_select; ++have) {
-                uint64_t best = 0;
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (x[j][e] > -INFINITY) {
-                            const uint64_t k = make_key(x[j][e], token0 + 4 * (tid + kThreads * j) + e - lead);
-                            if (k < last && k > best) best = k;
-                        }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const uint64_t k = __shfl_xor_sync(0xffffffffu, best, o);
-                    if (k > best) best = k;
-                }
-                if (lane == 0) sh.warp_key[warp] = best;
-                __syncthreads();
-                for (int w = 0; w < 8; ++w)
-                    if (sh.warp_key[w] > best) best = sh.warp_key[w];
-                __syncthreads();
-                if (best == 0) break;
-                if (tid == 0) keys[have] = best;
-                last = best;
-            }
-        }
-        for (uint32_t i = have + tid; i < p.n_select; i += kThreads) keys[i] = 0;
+    const uint32_t group = blockIdx.x / p.ctas_per_group;
+    const uint32_t unit = (blockIdx.x - group * p.ctas_per_group) * kWarps + warp;   // (beam, segment) of the group
+    if (unit < p.beams * p.segments) {
+        const uint32_t row = group * p.beams + unit / p.segments;
+        if (!p.finished || !p.finished[row]) segment(p, sh.list[warp], &sh.listed[warp], sh.part[warp], row, unit % p.segments, lane);
     }
-    // the last CTA of the group joins
-    __threadfence();
+    // the last CTA of the group joins: thread 0 publishes what the CTA wrote, and sees what the others published
     __syncthreads();
-    if (tid == 0) sh.last = atomicAdd(&p.counters[group], 1u) == p.beams * p.chunks - 1 ? 1u : 0u;
+    if (tid == 0) {
+        __threadfence();
+        sh.last = atomicAdd(&p.counters[group], 1u) == p.ctas_per_group - 1 ? 1u : 0u;
+        __threadfence();
+    }
     __syncthreads();
     if (!sh.last) return;
-    __threadfence();
     if (tid == 0) p.counters[group] = 0;
     join_group(p, sh, group);
 }
@@ -348,26 +469,26 @@ int beam_select(mlc_ctx* ctx, const void* logits, const void* cum, const void* f
     if (groups == 0 || beams == 0 || vocab == 0 || n_select == 0) return ctx->fail(MLC_ERR_INVALID_ARG, "zero dimension");
     if (beams > kMaxBeams || n_select > kMaxSelect)
         return ctx->fail(MLC_ERR_UNSUPPORTED, "more than %u beams or %u selected candidates", kMaxBeams, kMaxSelect);
-    if (vocab >= (size_t(1) << 31) || groups >= (size_t(1) << 24)) return ctx->fail(MLC_ERR_UNSUPPORTED, "dimension too large");
+    if (vocab >= (size_t(1) << 30) || groups >= (size_t(1) << 24)) return ctx->fail(MLC_ERR_UNSUPPORTED, "dimension too large");
     if (finished && pad_token >= vocab) return ctx->fail(MLC_ERR_INVALID_ARG, "pad token %u outside the vocabulary", pad_token);
     if (!aligned_to(logits, 4) || !aligned_to(cum, 4) || !aligned_to(out_scores, 4) || !aligned_to(out_parents, 4) ||
         !aligned_to(out_tokens, 4))
         return ctx->fail(MLC_ERR_INVALID_ARG, "buffers must be aligned to their elements");
     if (group_rows == 0 || group_rows > vocab) group_rows = vocab;
-    const size_t rows = groups * beams, parts = (vocab + group_rows - 1) / group_rows;
-    int nv = 8;
-    size_t per_part = 0;
-    for (;; nv /= 2) {   // shorter chunks while they are needed to give every SM one
-        const size_t most = static_cast<size_t>(nv) * kThreads * 4 - 4;   // an unaligned row takes a vector more
-        per_part = (group_rows + most - 1) / most;
-        if (nv == 2 || rows * parts * per_part >= static_cast<size_t>(ctx->sm_count)) break;
-    }
-    const size_t chunks = parts * per_part;
-    const size_t chunk_len = ((group_rows + per_part - 1) / per_part + 3) / 4 * 4;
-    if (rows * chunks >= (size_t(1) << 31) || beams * chunks * n_select >= (size_t(1) << 31))
+    const size_t rows = groups * beams, blocks = (vocab + group_rows - 1) / group_rows;
+    // Segments: enough to give every SM its warps once (twice as many take 68 us instead of 63), but no more lists per group than one CTA joins in a few
+    // microseconds, and at least a step each.
+    const size_t wanted = std::min<size_t>(static_cast<size_t>(ctx->sm_count) * kCtasPerSm * kWarps / rows, kMaxLists / beams);
+    size_t per_block = std::min<size_t>(std::max<size_t>(wanted / blocks, 1), (group_rows + kStep - 1) / kStep);
+    const size_t segment_len = ((group_rows + per_block - 1) / per_block + 3) / 4 * 4;
+    per_block = (group_rows + segment_len - 1) / segment_len;
+    const size_t segments = blocks * per_block;
+    const size_t ctas_per_group = (beams * segments + kWarps - 1) / kWarps;
+    if (rows * segments >= (size_t(1) << 31) || groups * ctas_per_group >= (size_t(1) << 31) ||
+        beams * segments * n_select >= (size_t(1) << 31))
         return ctx->fail(MLC_ERR_UNSUPPORTED, "too many rows");
     DeviceGuard guard(ctx->device);
-    const size_t key_bytes = rows * chunks * n_select * 8, sum_bytes = rows * chunks * sizeof(float2);
+    const size_t key_bytes = rows * segments * n_select * 8, sum_bytes = rows * segments * sizeof(float2);
     int st = ensure_op_scratch(ctx, ctx->beam_scratch, key_bytes + sum_bytes, "beam selection scratch");
     if (st == MLC_OK) st = ensure_op_scratch(ctx, ctx->beam_counters, groups * 4, "beam selection counters");
     if (st != MLC_OK) return st;
@@ -385,14 +506,13 @@ int beam_select(mlc_ctx* ctx, const void* logits, const void* cum, const void* f
     p.beams = static_cast<uint32_t>(beams);
     p.vocab = static_cast<uint32_t>(vocab);
     p.group_rows = static_cast<uint32_t>(group_rows);
-    p.chunks_per_part = static_cast<uint32_t>(per_part);
-    p.chunks = static_cast<uint32_t>(chunks);
-    p.chunk_len = static_cast<uint32_t>(chunk_len);
+    p.per_block = static_cast<uint32_t>(per_block);
+    p.segments = static_cast<uint32_t>(segments);
+    p.segment_len = static_cast<uint32_t>(segment_len);
+    p.ctas_per_group = static_cast<uint32_t>(ctas_per_group);
     p.n_select = static_cast<uint32_t>(n_select);
     p.pad = pad_token;
-    const dim3 grid(static_cast<unsigned>(rows * chunks));
-    auto kernel = nv == 8 ? beam_select_kernel<8> : nv == 4 ? beam_select_kernel<4> : beam_select_kernel<2>;
-    MLCB_CUDA(ctx, launch_dependent(ctx, kernel, grid, kThreads, 0, p));
+    MLCB_CUDA(ctx, launch_dependent(ctx, beam_select_kernel, dim3(static_cast<unsigned>(groups * ctas_per_group)), kThreads, 0, p));
     ++ctx->launches;
     return MLC_OK;
 }

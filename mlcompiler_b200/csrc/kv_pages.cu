@@ -18,7 +18,7 @@ namespace mlcb {
 namespace {
 
 constexpr uint32_t kMaxPools = 128;      // per launch; a call with more takes several
-constexpr uint32_t kInlinePairs = 240;   // (source, destination) pairs that travel as kernel parameters
+constexpr uint32_t kInlinePairs = 128;   // (source, destination) pairs that travel as kernel parameters
 
 struct CopyParams {
     char* pools[kMaxPools];
@@ -28,23 +28,33 @@ struct CopyParams {
     uint32_t n_pairs;
 };
 
+constexpr uint32_t kBatch = 8;   // vectors a thread has in flight
+
+// Launched as a programmatic dependent of the kernel in front; it does not let its own dependents go before it is done, so
+// that nothing behind it reads a page early.
 template <typename Vec>
-__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams p, uint32_t chunks, uint32_t chunk_vecs) {
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams p, uint32_t chunks) {
     const uint32_t pair_i = blockIdx.x / chunks, chunk = blockIdx.x - pair_i * chunks;
     const uint2 pair = p.pairs ? p.pairs[pair_i] : p.inline_pairs[pair_i];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (pair.x == pair.y) return;
     char* pool = p.pools[blockIdx.y];
     const Vec* src = reinterpret_cast<const Vec*>(pool + static_cast<uint64_t>(pair.x) * p.unit_bytes);
     Vec* dst = reinterpret_cast<Vec*>(pool + static_cast<uint64_t>(pair.y) * p.unit_bytes);
-    const uint64_t n = p.unit_bytes / sizeof(Vec);
-    const uint64_t first = static_cast<uint64_t>(chunk) * chunk_vecs;
-    const uint64_t end = first + chunk_vecs < n ? first + chunk_vecs : n;
-    for (uint64_t i = first + threadIdx.x; i < end; i += 256) dst[i] = src[i];
+    const uint64_t n = p.unit_bytes / sizeof(Vec), first = static_cast<uint64_t>(chunk) * (256 * kBatch) + threadIdx.x;
+    Vec v[kBatch];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i)
+        if (first + 256 * i < n) v[i] = src[first + 256 * i];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i)
+        if (first + 256 * i < n) dst[first + 256 * i] = v[i];
 }
 
 // Rows of one request move from rising source rows to rising destination rows, never upwards (destination <= source in
 // token order). A thread owns one column of the row in one pool and works through the request's moves in order, so a row
-// is always read before a later move can write it, whatever the other threads do.
+// is always read before a later move can write it, whatever the other threads do. It has kBatch rows in flight: the rows it has not
+// read yet lie behind every destination of the batch.
 struct MoveParams {
     char* pools[kMaxPools];
     const uint2* moves;                  // device list, or null: `inline_moves`
@@ -63,9 +73,21 @@ __global__ void __launch_bounds__(128) move_rows_kernel(const __grid_constant__ 
     char* pool = p.pools[blockIdx.y] + static_cast<uint64_t>(column) * sizeof(Vec);
     const uint32_t* first = p.first ? p.first : p.inline_first;
     const uint2* moves = p.moves ? p.moves : p.inline_moves;
-    for (uint32_t i = first[req], end = first[req + 1]; i < end; ++i) {
-        const uint2 m = moves[i];
-        *reinterpret_cast<Vec*>(pool + m.y * p.row_bytes) = *reinterpret_cast<const Vec*>(pool + m.x * p.row_bytes);
+    const uint32_t end = first[req + 1];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (uint32_t i = first[req]; i < end; i += kBatch) {
+        Vec v[kBatch];
+        uint32_t to[kBatch];
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            if (i + k < end) {
+                const uint2 m = moves[i + k];
+                to[k] = m.y;
+                v[k] = *reinterpret_cast<const Vec*>(pool + m.x * p.row_bytes);
+            }
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            if (i + k < end) *reinterpret_cast<Vec*>(pool + to[k] * p.row_bytes) = v[k];
     }
 }
 
@@ -179,22 +201,22 @@ int copy_pages(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, cons
     p.unit_bytes = page_bytes;
     p.n_pairs = static_cast<uint32_t>(n_pairs);
     const uint32_t vec = vector_bytes(pools, n_pools, page_bytes);
-    const uint32_t chunk_vecs = 256 * 8;
-    const uint64_t chunks = (page_bytes / vec + chunk_vecs - 1) / chunk_vecs;
+    const uint64_t chunks = (page_bytes / vec + 256 * kBatch - 1) / (256 * kBatch);
     if (chunks * n_pairs >= (uint64_t(1) << 31)) return ctx->fail(MLC_ERR_UNSUPPORTED, "too many pages in one call");
     for (size_t p0 = 0; p0 < n_pools; p0 += kMaxPools) {
         const size_t n = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;
         for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
         const dim3 grid(static_cast<unsigned>(chunks * n_pairs), static_cast<unsigned>(n));
         const uint32_t c = static_cast<uint32_t>(chunks);
+        cudaError_t e;
         switch (vec) {
-            case 16: copy_pages_kernel<uint4><<<grid, 256, 0, ctx->stream>>>(p, c, chunk_vecs); break;
-            case 8: copy_pages_kernel<uint2><<<grid, 256, 0, ctx->stream>>>(p, c, chunk_vecs); break;
-            case 4: copy_pages_kernel<uint32_t><<<grid, 256, 0, ctx->stream>>>(p, c, chunk_vecs); break;
-            default: copy_pages_kernel<uint16_t><<<grid, 256, 0, ctx->stream>>>(p, c, chunk_vecs); break;
+            case 16: e = launch_dependent(ctx, copy_pages_kernel<uint4>, grid, 256, 0, p, c); break;
+            case 8: e = launch_dependent(ctx, copy_pages_kernel<uint2>, grid, 256, 0, p, c); break;
+            case 4: e = launch_dependent(ctx, copy_pages_kernel<uint32_t>, grid, 256, 0, p, c); break;
+            default: e = launch_dependent(ctx, copy_pages_kernel<uint16_t>, grid, 256, 0, p, c); break;
         }
+        MLCB_CUDA(ctx, e);
         ++ctx->launches;
-        MLCB_CUDA(ctx, cudaGetLastError());
     }
     note_pool_writes(ctx, pools, n_pools);
     return sync ? wait_for_copy(ctx, "page copy") : MLC_OK;
@@ -274,14 +296,15 @@ int compact_rows(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, co
         for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
         const dim3 grid(static_cast<unsigned>((threads + 127) / 128), static_cast<unsigned>(n));
         const uint32_t v = static_cast<uint32_t>(vecs);
+        cudaError_t e;
         switch (vec) {
-            case 16: move_rows_kernel<uint4><<<grid, 128, 0, ctx->stream>>>(p, v, threads); break;
-            case 8: move_rows_kernel<uint2><<<grid, 128, 0, ctx->stream>>>(p, v, threads); break;
-            case 4: move_rows_kernel<uint32_t><<<grid, 128, 0, ctx->stream>>>(p, v, threads); break;
-            default: move_rows_kernel<uint16_t><<<grid, 128, 0, ctx->stream>>>(p, v, threads); break;
+            case 16: e = launch_dependent(ctx, move_rows_kernel<uint4>, grid, 128, 0, p, v, threads); break;
+            case 8: e = launch_dependent(ctx, move_rows_kernel<uint2>, grid, 128, 0, p, v, threads); break;
+            case 4: e = launch_dependent(ctx, move_rows_kernel<uint32_t>, grid, 128, 0, p, v, threads); break;
+            default: e = launch_dependent(ctx, move_rows_kernel<uint16_t>, grid, 128, 0, p, v, threads); break;
         }
+        MLCB_CUDA(ctx, e);
         ++ctx->launches;
-        MLCB_CUDA(ctx, cudaGetLastError());
     }
     note_pool_writes(ctx, pools, n_pools);
     return sync ? wait_for_copy(ctx, "row compaction") : MLC_OK;

@@ -688,6 +688,10 @@ int mlc_page_pool_allocate_n(mlc_page_pool* pool, size_t n, uint32_t* out /* [n]
 /* release: the reference asserts on a bad id (paged_kv.cpp:37-42); this returns 0 and
  * changes nothing. */
 int mlc_page_pool_release(mlc_page_pool* pool, uint32_t page_id);
+/* Shared pages (no counterpart in the reference, whose pages have one owner). share adds an owner to a page in
+ * use (0 if it is not); release takes one away, and frees the page with the last. owners: 0 = free. */
+int mlc_page_pool_share(mlc_page_pool* pool, uint32_t page_id);
+uint32_t mlc_page_pool_owners(const mlc_page_pool* pool, uint32_t page_id);
 uint32_t mlc_page_pool_capacity(const mlc_page_pool* pool);
 size_t mlc_page_pool_in_use(const mlc_page_pool* pool);
 size_t mlc_page_pool_free(const mlc_page_pool* pool);
@@ -699,6 +703,15 @@ void mlc_kv_state_destroy(mlc_kv_state* state);
 int mlc_kv_state_reserve(mlc_kv_state* state, mlc_page_pool* pool, size_t target_tokens);
 int mlc_kv_state_extend_one_token(mlc_kv_state* state, mlc_page_pool* pool, uint32_t* page_id,
                                   uint32_t* slot_in_page);
+/* Several continuations of one request. fork: `state`, which has no pages, becomes a second owner of all of
+ * `parent`'s. extend_one_token fails where it would write into a page with other owners; the _owned form takes a
+ * new page in its place and returns 2 with the copy that is owed before anything is written there (copy_dst
+ * becomes a copy of copy_src: mlc_encode_copy_kv_pages), 1 if none is, 0 on failure. truncate keeps the first
+ * `tokens` tokens and releases the pages behind them (0 if there are fewer tokens): what a rejected draft took. */
+int mlc_kv_state_fork(mlc_kv_state* state, const mlc_kv_state* parent, mlc_page_pool* pool);
+int mlc_kv_state_extend_one_token_owned(mlc_kv_state* state, mlc_page_pool* pool, uint32_t* page_id, uint32_t* slot_in_page,
+                                        uint32_t* copy_src, uint32_t* copy_dst);
+int mlc_kv_state_truncate(mlc_kv_state* state, mlc_page_pool* pool, size_t tokens);
 int mlc_kv_state_locate(const mlc_kv_state* state, size_t pos, uint32_t* page_id, uint32_t* slot_in_page);
 void mlc_kv_state_release_all(mlc_kv_state* state, mlc_page_pool* pool);
 size_t mlc_kv_state_total_tokens(const mlc_kv_state* state);
@@ -871,6 +884,22 @@ size_t mlc_executor_run_decode(mlc_executor* exec, const mlc_request_slot* slots
  * instead of batch * vocab_size floats. Returns n, or 0 when the executor cannot do it (nothing has run
  * then: use mlc_executor_run_decode). The scheduler uses this path by itself. */
 size_t mlc_executor_run_decode_greedy(mlc_executor* exec, const mlc_request_slot* slots, size_t n, uint64_t* tokens);
+/* The same pass ending in a selection step of beam search (mlc_encode_beam_select) on the device: slots [g * beams,
+ * (g + 1) * beams) are the beams of group g, cum_scores and finished (may be NULL) host arrays with an entry per
+ * slot. scores, parents and tokens receive n_select entries per group, as described there. Returns n, or 0 when the
+ * executor cannot do it or the pass failed. */
+size_t mlc_executor_run_decode_beams(mlc_executor* exec, const mlc_request_slot* slots, size_t n, size_t beams,
+                                     const float* cum_scores, const uint8_t* finished, size_t n_select, uint32_t pad_token,
+                                     float* scores, uint32_t* parents, uint32_t* tokens);
+/* Several continuations of one request in the executor (mlc_status; no counterpart in the reference).
+ *   fork_request      child_id, which must have no pages, continues from where parent_id is: it shares the parent's
+ *                     pages, and the first pass that writes into a shared page copies it, in every layer, first
+ *   truncate_request  forgets the tokens behind the first `tokens` and releases their pages
+ *   assign_beams      request_ids[i] continues from where request_ids[parents[i]] is now, for all i at once - the
+ *                     reordering after a selection step; every id must have pages and be named once */
+int mlc_executor_fork_request(mlc_executor* exec, uint32_t parent_id, uint32_t child_id);
+int mlc_executor_truncate_request(mlc_executor* exec, uint32_t request_id, size_t tokens);
+int mlc_executor_assign_beams(mlc_executor* exec, const uint32_t* request_ids, const uint32_t* parents, size_t n);
 /* run_prefill: returns the number of logits (0 = failed). */
 size_t mlc_executor_run_prefill(mlc_executor* exec, uint32_t request_id, const uint64_t* tokens, size_t n,
                                 float* logits, size_t capacity);

@@ -167,11 +167,18 @@ def _ptr(x) -> int:
     raise TypeError(f"not a device buffer: {type(x)}")
 
 
+_U32 = np.dtype(np.uint32)
+
+
 def _u32_at(a):
-    """Like _u32, with the address as an integer: what the calls of a step's hot path pass."""
-    if type(a) is not np.ndarray or a.dtype != np.uint32 or not a.flags.c_contiguous:
+    """Like _u32, with the address as an integer: for the calls of a step's hot path. (An array's ctypes attribute takes three
+    times as long as a buffer's address; it is left for empty and read-only arrays, which have none.)"""
+    if type(a) is not np.ndarray or a.dtype is not _U32 or not a.flags.c_contiguous:
         a = np.ascontiguousarray(np.asarray(a, dtype=np.uint32))
-    return a, a.ctypes.data
+    try:
+        return a, C.addressof(C.c_char.from_buffer(a))
+    except (TypeError, ValueError, BufferError):
+        return a, a.ctypes.data
 
 
 def _u32(a):

@@ -5,6 +5,7 @@
 #include "ctx.hpp"
 
 #include <cstring>
+#include <unordered_set>
 
 namespace mlcb {
 namespace runtime {
@@ -99,6 +100,59 @@ bool PagedAttentionExecutor::assume_context(uint32_t request_id, size_t tokens) 
     return true;
 }
 
+bool PagedAttentionExecutor::fork_request(uint32_t parent, uint32_t child) {
+    const auto from = requests_.find(parent);
+    if (!pool_ || parent == child || from == requests_.end() || !from->second.page_state || from->second.page_state->page_table.empty())
+        return false;
+    if (page_state(child) && !page_state(child)->page_table.empty()) return false;
+    std::unique_ptr<RequestKVState> state(new RequestKVState());
+    state->request_id = child;
+    if (!state->fork_from(*from->second.page_state, *pool_)) return false;
+    const size_t position = from->second.next_position;
+    PerRequest& req = ensure_request(child);   // may move the parent's entry
+    req.page_state = std::move(state);
+    req.next_position = position;
+    return true;
+}
+
+bool PagedAttentionExecutor::truncate_request(uint32_t request_id, size_t tokens) {
+    const auto it = requests_.find(request_id);
+    if (!pool_ || it == requests_.end() || !it->second.page_state || !it->second.page_state->truncate(*pool_, tokens)) return false;
+    it->second.next_position = tokens;
+    return true;
+}
+
+bool PagedAttentionExecutor::assign_beams(const std::vector<uint32_t>& ids, const std::vector<uint32_t>& parents) {
+    const size_t n = ids.size();
+    if (!pool_ || parents.size() != n) return false;
+    std::unordered_set<uint32_t> seen;
+    for (size_t i = 0; i < n; ++i) {
+        if (parents[i] >= n || !seen.insert(ids[i]).second) return false;
+        const RequestKVState* s = page_state(ids[i]);
+        if (!s || s->page_table.empty()) return false;
+    }
+    // every new state takes its share of the old ones before any of them is given up
+    std::vector<std::unique_ptr<RequestKVState>> states(n);
+    std::vector<size_t> positions(n);
+    for (size_t i = 0; i < n; ++i) {
+        const PerRequest& from = requests_[ids[parents[i]]];
+        states[i].reset(new RequestKVState());
+        states[i]->request_id = ids[i];
+        if (!states[i]->fork_from(*from.page_state, *pool_)) {
+            for (size_t k = 0; k < i; ++k) states[k]->release_all(*pool_);
+            return false;
+        }
+        positions[i] = from.next_position;
+    }
+    for (size_t i = 0; i < n; ++i) requests_[ids[i]].page_state->release_all(*pool_);
+    for (size_t i = 0; i < n; ++i) {
+        PerRequest& req = requests_[ids[i]];
+        req.page_state = std::move(states[i]);
+        req.next_position = positions[i];
+    }
+    return true;
+}
+
 void PagedAttentionExecutor::release_request(uint32_t request_id) {
     auto it = requests_.find(request_id);
     if (it == requests_.end()) return;
@@ -146,6 +200,18 @@ bool PagedAttentionExecutor::run_decode_greedy(const std::vector<RequestSlot>& s
     }
     for (size_t i = 0; i < slots.size(); ++i)
         if (!out.per_request[i].success) tokens[i] = UINT64_MAX;
+    return true;
+}
+
+bool PagedAttentionExecutor::run_decode_beams(const std::vector<RequestSlot>& slots, const BeamStep& beam) {
+    if (slots.empty() || !storage_ || !pool_ || !model_ || order_ != CallOrder::Fused) return false;
+    if (!beam.beams || slots.size() % beam.beams || !beam.n_select || !beam.cum_scores || !beam.scores || !beam.parents || !beam.tokens)
+        return false;
+    if (beam.beams > 64 || beam.n_select > 64 || (beam.finished && beam.pad_token >= model_->vocab_size)) return false;   // as the selection does
+    const BatchedDecodeOutput out = walker_->step(slots, nullptr, nullptr, &beam);
+    if (out.per_request.size() != slots.size()) return false;
+    for (const auto& p : out.per_request)
+        if (!p.success) return false;
     return true;
 }
 

@@ -143,12 +143,33 @@ public:
     // already has pages or the pool cannot supply them.
     bool assume_context(uint32_t request_id, size_t tokens);
     const RequestKVState* page_state(uint32_t request_id) const;
+    // A second continuation of a request (no counterpart in the reference): `child`, which must not have pages yet, shares the
+    // parent's pages and position. A page that both own is copied by the first pass that writes into it. False if the
+    // parent has no pages or the child has some.
+    bool fork_request(uint32_t parent, uint32_t child);
+    // Forgets the tokens of a request behind the first `tokens`, and the pages they took. False if there are fewer.
+    bool truncate_request(uint32_t request_id, size_t tokens);
+    // Request ids[i] continues from where ids[parents[i]] is now, for all i at once: the reordering after a selection
+    // step of beam search. False (and nothing changed) if an id is named twice or has no pages, or a parent is out of range.
+    bool assign_beams(const std::vector<uint32_t>& ids, const std::vector<uint32_t>& parents);
 
     BatchedDecodeOutput run_decode(const std::vector<RequestSlot>& slots) override;
     // The same pass with a model attached, the logits written to the caller's rows (row r at logits + r * stride
     // floats, stride >= vocabulary size) instead of into per-request vectors; straight from the device when the
     // buffer is page-locked memory. The returned entries carry request ids and success flags only.
     BatchedDecodeOutput run_decode_into(const std::vector<RequestSlot>& slots, float* logits, size_t stride);
+    // A decode pass that ends in a selection step of beam search on the device: slots [g * beams, (g + 1) * beams) are the
+    // beams of group g. The three outputs hold n_select entries per group. False (nothing has run) without a model or in
+    // the reference's call order, or if the pass failed.
+    struct BeamStep {
+        size_t beams = 0, n_select = 0;
+        const float* cum_scores = nullptr;      // [slots]
+        const uint8_t* finished = nullptr;      // [slots], may be null
+        uint32_t pad_token = 0;
+        float* scores = nullptr;
+        uint32_t *parents = nullptr, *tokens = nullptr;
+    };
+    bool run_decode_beams(const std::vector<RequestSlot>& slots, const BeamStep& beam);
     size_t logits_per_request() const;
     std::vector<float> run_prefill(uint32_t request_id, const std::vector<uint64_t>& tokens) override;
     void release_request(uint32_t request_id) override;

@@ -45,8 +45,29 @@ static double now_us() {
     return std::chrono::duration<double, std::micro>(std::chrono::steady_clock::now().time_since_epoch()).count();
 }
 
+bool BatchedWalker::copy_shared_pages(const PageCopies& copies) {
+    if (copies.empty()) return true;
+    PagedAttentionExecutor& ex = exec_;
+    const PagedKVStorage* storage = ex.storage_;
+    copy_pools_.clear();
+    for (uint32_t layer = 0; layer < storage->n_layers(); ++layer) {
+        copy_pools_.push_back(storage->k_buffer(layer));
+        copy_pools_.push_back(storage->v_buffer(layer));
+    }
+    copy_src_.clear();
+    copy_dst_.clear();
+    for (const auto& c : copies) {
+        copy_src_.push_back(c.first);
+        copy_dst_.push_back(c.second);
+    }
+    return mlc_pass_begin(ex.ctx_) == MLC_OK &&
+           mlc_encode_copy_kv_pages(ex.ctx_, copy_pools_.data(), copy_pools_.size(), copy_src_.data(), copy_dst_.data(), copies.size(),
+                                    storage->page_size_tokens(), storage->n_kv_heads(), storage->head_dim(), storage->dtype_bytes(),
+                                    storage->capacity_pages()) == MLC_OK;
+}
+
 BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, const LogitsSink* sink,
-                                        std::vector<uint64_t>* greedy) {
+                                        std::vector<uint64_t>* greedy, const PagedAttentionExecutor::BeamStep* beam) {
     BatchedDecodeOutput out;
     if (slots.empty()) return out;
     NvtxRange pass_range("mlc decode pass");
@@ -56,7 +77,12 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
     PagedKVStorage* storage = ex.storage_;
     const size_t N = slots.size();
     const uint32_t H = ex.H_, KVH = ex.KVH_, D = ex.D_, P = storage->page_size_tokens();
+    PageCopies copies;
+    bool copied = false;
     auto fail_all = [&]() {
+        // a page table already names the copies: they are made even if the pass is not
+        if (!copied) copied = copy_shared_pages(copies);
+        if (!copies.empty()) mlc_pass_flush(ctx);
         out.per_request.clear();
         for (const auto& s : slots) {
             BatchedDecodeOutput::PerRequest p;
@@ -78,10 +104,15 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
             reqs[r]->page_state->request_id = slots[r].request_id;
             reqs[r]->page_state->page_size_tokens = ex.page_size_tokens_;
         }
-        auto loc = reqs[r]->page_state->extend_one_token(*ex.pool_);
+        auto loc = reqs[r]->page_state->extend_one_token(*ex.pool_, &copies);
         if (!loc) return fail_all();
         page_ids[r] = loc->first;
         slot_ids[r] = loc->second;
+    }
+
+    if (!(copied = copy_shared_pages(copies))) {
+        copied = true;   // not a second time
+        return fail_all();
     }
 
     // Tables of the pass, built once (the reference rebuilds them per layer, 316-325):
@@ -126,18 +157,20 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
             direct = cudaPointerGetAttributes(&attr, sink->dst) == cudaSuccess && attr.type == cudaMemoryTypeHost;
             cudaGetLastError();   // a pointer the runtime does not know is not an error here
         }
-        if (greedy && tokens_pinned_count_ < N) {
+        // token ids of greedy sampling, or scores, parents and tokens of a beam step
+        const size_t selected = beam ? N / beam->beams * beam->n_select : 0, words = beam ? 3 * selected : greedy ? N : 0;
+        if (tokens_pinned_count_ < words) {
             if (tokens_pinned_) cudaFreeHost(tokens_pinned_);
             tokens_pinned_ = nullptr;
             tokens_pinned_count_ = 0;
             DeviceGuard guard(ctx->device);
-            if (cudaHostAlloc(reinterpret_cast<void**>(&tokens_pinned_), std::max<size_t>(N, 64) * sizeof(uint32_t),
+            if (cudaHostAlloc(reinterpret_cast<void**>(&tokens_pinned_), std::max<size_t>(words, 64) * sizeof(uint32_t),
                               cudaHostAllocDefault) != cudaSuccess)
                 return fail_all();
-            tokens_pinned_count_ = std::max<size_t>(N, 64);
+            tokens_pinned_count_ = std::max<size_t>(words, 64);
             ++ctx->allocations;
         }
-        if (!greedy && !direct && logits_pinned_floats_ < N * vocab) {
+        if (!greedy && !beam && !direct && logits_pinned_floats_ < N * vocab) {
             if (logits_pinned_) cudaFreeHost(logits_pinned_);
             logits_pinned_ = nullptr;
             logits_pinned_floats_ = 0;
@@ -153,12 +186,16 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
         ok = ok && encode_model_pass(slots, plan, page_ids, slot_ids, pt_flat, pt_off, seq_lens, q_pos,
                                      direct ? sink->dst : logits_pinned_, direct ? sink->stride : vocab, 0,
                                      true,   // a decode pass writes one row per request, at the plan's (page, slot)
-                                     greedy ? tokens_pinned_ : nullptr);
+                                     greedy || beam ? tokens_pinned_ : nullptr, beam);
         const double t_enc = walker_trace() ? now_us() : 0.0;
         ok = (mlc_pass_flush(ctx) == MLC_OK) && ok;   // the logits are on the host when this returns
         const double t_flush = walker_trace() ? now_us() : 0.0;
         if (!ok) return fail_all();
-        if (greedy) {
+        if (beam) {
+            std::memcpy(beam->scores, tokens_pinned_, selected * sizeof(uint32_t));
+            std::memcpy(beam->parents, tokens_pinned_ + selected, selected * sizeof(uint32_t));
+            std::memcpy(beam->tokens, tokens_pinned_ + 2 * selected, selected * sizeof(uint32_t));
+        } else if (greedy) {
             greedy->assign(tokens_pinned_, tokens_pinned_ + N);
         } else if (!direct && sink && sink->dst && sink->stride >= vocab) {
             for (size_t r = 0; r < N; ++r)
@@ -170,7 +207,7 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
             BatchedDecodeOutput::PerRequest p;
             p.request_id = slots[r].request_id;
             p.success = true;
-            if (!to_sink && !greedy) p.logits.assign(logits_pinned_ + r * vocab, logits_pinned_ + (r + 1) * vocab);
+            if (!to_sink && !greedy && !beam) p.logits.assign(logits_pinned_ + r * vocab, logits_pinned_ + (r + 1) * vocab);
             reqs[r]->next_position = slots[r].sequence_position + 1;
             out.per_request.push_back(std::move(p));
         }
@@ -267,7 +304,8 @@ bool BatchedWalker::encode_model_pass(const std::vector<RequestSlot>& slots, mlc
                                       const std::vector<uint32_t>& pt_flat, const std::vector<uint32_t>& pt_off,
                                       const std::vector<uint32_t>& seq_lens, const std::vector<uint32_t>& q_pos,
                                       float* logits_host, size_t logits_stride, size_t head_first,
-                                      bool rows_per_request_only, uint32_t* greedy_host) {
+                                      bool rows_per_request_only, uint32_t* greedy_host,
+                                      const PagedAttentionExecutor::BeamStep* beam) {
     PagedAttentionExecutor& ex = exec_;
     mlc_ctx* ctx = ex.ctx_;
     PagedKVStorage* storage = ex.storage_;
@@ -427,6 +465,17 @@ bool BatchedWalker::encode_model_pass(const std::vector<RequestSlot>& slots, mlc
                               cudaMemcpyDeviceToHost, ctx->d2h_stream) != cudaSuccess)
             return false;
     }
+    if (beam) {
+        // a selection step of beam search on the device: three words per selected candidate come back
+        const size_t n_groups = head_n / beam->beams, selected = n_groups * beam->n_select;
+        uint32_t* res = static_cast<uint32_t*>(scratch("w_beams", 3 * selected * sizeof(uint32_t)));
+        const void* cum = stage_to_device(ctx, beam->cum_scores, head_n * sizeof(float));
+        const void* done = beam->finished ? stage_to_device(ctx, beam->finished, head_n) : nullptr;
+        return res && cum && (done || !beam->finished) &&
+               mlc_encode_beam_select(ctx, logits, cum, done, n_groups, beam->beams, vocab, group_rows, beam->n_select,
+                                      beam->pad_token, res, res + selected, res + 2 * selected) == MLC_OK &&
+               cudaMemcpyAsync(greedy_host, res, 3 * selected * sizeof(uint32_t), cudaMemcpyDeviceToHost, ctx->stream) == cudaSuccess;
+    }
     if (greedy_host) {
         // greedy sampling on the device: one token id per request comes back instead of the logits
         void* ids = scratch("w_argmax", head_n * sizeof(uint32_t));
@@ -472,13 +521,19 @@ std::vector<float> BatchedWalker::prefill_model(uint32_t request_id, const std::
         // far stay with the request until it is released, as in the token loop.
         std::vector<uint32_t> page_ids(n), slot_ids(n), seq_lens(n), q_pos(n), pt_off(n + 1, 0), pt_flat;
         std::vector<RequestSlot> slots(n);
+        PageCopies copies;   // of a shared last page, made at once: at most one for a prompt
+        auto finish_copies = [&] { return copies.empty() || (copy_shared_pages(copies) && mlc_pass_flush(ctx) == MLC_OK); };
         for (size_t i = 0; i < n; ++i) {
-            auto loc = req.page_state->extend_one_token(*ex.pool_);
-            if (!loc) return {};
+            auto loc = req.page_state->extend_one_token(*ex.pool_, &copies);
+            if (!loc) {
+                finish_copies();
+                return {};
+            }
             page_ids[i] = loc->first;
             slot_ids[i] = loc->second;
             slots[i] = RequestSlot{request_id, tokens[done + i], cursor + done + i};
         }
+        if (!finish_copies()) return {};
         const std::vector<uint32_t>& table = req.page_state->page_table;
         for (size_t i = 0; i < n; ++i) {
             q_pos[i] = static_cast<uint32_t>(cursor + done + i);
@@ -525,13 +580,19 @@ std::vector<float> BatchedWalker::prefill(uint32_t request_id, const std::vector
     // pages taken so far stay with the request until it is released, as in the token loop
     std::vector<uint32_t> page_ids(n), slot_ids(n);
     std::vector<RequestSlot> slots(n);
+    PageCopies copies;
+    auto finish_copies = [&] { return copies.empty() || (copy_shared_pages(copies) && mlc_pass_flush(ctx) == MLC_OK); };
     for (size_t i = 0; i < n; ++i) {
-        auto loc = req.page_state->extend_one_token(*ex.pool_);
-        if (!loc) return {};
+        auto loc = req.page_state->extend_one_token(*ex.pool_, &copies);
+        if (!loc) {
+            finish_copies();
+            return {};
+        }
         page_ids[i] = loc->first;
         slot_ids[i] = loc->second;
         slots[i] = RequestSlot{request_id, tokens[i], cursor + i};
     }
+    if (!finish_copies()) return {};
     const std::vector<uint32_t>& table = req.page_state->page_table;
     const uint32_t pt_off[2] = {0u, static_cast<uint32_t>(table.size())};
     const uint32_t seq_len = static_cast<uint32_t>(req.page_state->total_tokens());

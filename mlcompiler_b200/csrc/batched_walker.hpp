@@ -20,9 +20,11 @@ public:
         size_t stride = 0;
     };
     // greedy (model attached only): the pass ends with the argmax of every request's logits on the device and
-    // *greedy receives one token id per request; no logits come back.
+    // *greedy receives one token id per request; no logits come back. beam (the same way): the pass ends with a selection
+    // step of beam search, whose results go to the arrays it names.
     BatchedDecodeOutput step(const std::vector<RequestSlot>& slots, const LogitsSink* sink = nullptr,
-                             std::vector<uint64_t>* greedy = nullptr);
+                             std::vector<uint64_t>* greedy = nullptr,
+                             const PagedAttentionExecutor::BeamStep* beam = nullptr);
     // All tokens of a prompt chunk in one pass per layer: the chunk's K/V rows are scattered,
     // then chunked causal attention runs over the request's pages. Returns the last token's
     // attention output of the last layer, or {} on failure. The reference reaches the same
@@ -42,7 +44,11 @@ private:
                            const std::vector<uint32_t>& slot_ids, const std::vector<uint32_t>& pt_flat,
                            const std::vector<uint32_t>& pt_off, const std::vector<uint32_t>& seq_lens,
                            const std::vector<uint32_t>& q_pos, float* logits_host, size_t logits_stride, size_t head_first,
-                           bool rows_per_request_only, uint32_t* greedy_host);
+                           bool rows_per_request_only, uint32_t* greedy_host,
+                           const PagedAttentionExecutor::BeamStep* beam = nullptr);
+    // The copies that a pass's extensions owe (shared pages that it writes into), in every layer's pools, in front of the
+    // pass's kernels. Opens the pass.
+    bool copy_shared_pages(const PageCopies& copies);
 
     PagedAttentionExecutor& exec_;
     std::vector<float> cos_host_, sin_host_;
@@ -51,6 +57,8 @@ private:
     size_t logits_pinned_floats_ = 0;
     uint32_t* tokens_pinned_ = nullptr;   // page-locked landing area of the greedy token ids
     size_t tokens_pinned_count_ = 0;
+    std::vector<void*> copy_pools_;   // every layer's K and V pool
+    std::vector<uint32_t> copy_src_, copy_dst_;
     // host staging, reused across passes
     std::vector<float> q_host_;
     std::vector<uint16_t> k_host_, v_host_;

@@ -98,6 +98,8 @@ int mlc_page_pool_allocate_n(mlc_page_pool* p, size_t n, uint32_t* out) {
     return 1;
 }
 int mlc_page_pool_release(mlc_page_pool* p, uint32_t page_id) { return p && p->pool.release(page_id) ? 1 : 0; }
+int mlc_page_pool_share(mlc_page_pool* p, uint32_t page_id) { return p && p->pool.share(page_id) ? 1 : 0; }
+uint32_t mlc_page_pool_owners(const mlc_page_pool* p, uint32_t page_id) { return p ? p->pool.owners(page_id) : 0; }
 uint32_t mlc_page_pool_capacity(const mlc_page_pool* p) { return p ? p->pool.capacity() : 0; }
 size_t mlc_page_pool_in_use(const mlc_page_pool* p) { return p ? p->pool.pages_in_use() : 0; }
 size_t mlc_page_pool_free(const mlc_page_pool* p) { return p ? p->pool.pages_free() : 0; }
@@ -120,6 +122,34 @@ int mlc_kv_state_extend_one_token(mlc_kv_state* s, mlc_page_pool* p, uint32_t* p
     if (page_id) *page_id = loc->first;
     if (slot) *slot = loc->second;
     return 1;
+}
+int mlc_kv_state_extend_one_token_owned(mlc_kv_state* s, mlc_page_pool* p, uint32_t* page_id, uint32_t* slot, uint32_t* copy_src,
+                                        uint32_t* copy_dst) {
+    if (!s || !p || !page_id || !slot || !copy_src || !copy_dst) return 0;
+    try {
+        PageCopies copies;
+        const auto loc = s->st.extend_one_token(p->pool, &copies);
+        if (!loc) return 0;
+        *page_id = loc->first;
+        *slot = loc->second;
+        if (copies.empty()) return 1;
+        *copy_src = copies.front().first;
+        *copy_dst = copies.front().second;
+        return 2;
+    } catch (const std::exception&) {
+        return 0;
+    }
+}
+int mlc_kv_state_fork(mlc_kv_state* s, const mlc_kv_state* parent, mlc_page_pool* p) {
+    if (!s || !parent || !p) return 0;
+    try {
+        return s->st.fork_from(parent->st, p->pool) ? 1 : 0;
+    } catch (const std::exception&) {
+        return 0;
+    }
+}
+int mlc_kv_state_truncate(mlc_kv_state* s, mlc_page_pool* p, size_t tokens) {
+    return s && p && s->st.truncate(p->pool, tokens) ? 1 : 0;
 }
 int mlc_kv_state_locate(const mlc_kv_state* s, size_t pos, uint32_t* page_id, uint32_t* slot) {
     if (!s) return 0;
@@ -361,6 +391,49 @@ size_t mlc_executor_run_decode_greedy(mlc_executor* e, const mlc_request_slot* s
     if (!e->exec->run_decode_greedy(in, out) || out.size() != n) return 0;
     std::memcpy(tokens, out.data(), n * sizeof(uint64_t));
     return n;
+}
+size_t mlc_executor_run_decode_beams(mlc_executor* e, const mlc_request_slot* slots, size_t n, size_t beams, const float* cum_scores,
+                                     const uint8_t* finished, size_t n_select, uint32_t pad_token, float* scores, uint32_t* parents,
+                                     uint32_t* tokens) {
+    if (!e || !e->paged || (!slots && n)) return 0;
+    try {
+        std::vector<RequestSlot> in(n);
+        for (size_t i = 0; i < n; ++i)
+            in[i] = RequestSlot{slots[i].request_id, slots[i].input_token, static_cast<size_t>(slots[i].sequence_position)};
+        PagedAttentionExecutor::BeamStep b;
+        b.beams = beams;
+        b.n_select = n_select;
+        b.cum_scores = cum_scores;
+        b.finished = finished;
+        b.pad_token = pad_token;
+        b.scores = scores;
+        b.parents = parents;
+        b.tokens = tokens;
+        return e->paged->run_decode_beams(in, b) ? n : 0;
+    } catch (const std::exception&) {
+        return 0;
+    }
+}
+int mlc_executor_fork_request(mlc_executor* e, uint32_t parent_id, uint32_t child_id) {
+    if (!e || !e->paged) return MLC_ERR_INVALID_ARG;
+    try {
+        return e->paged->fork_request(parent_id, child_id) ? MLC_OK : MLC_ERR_INVALID_ARG;
+    } catch (const std::exception&) {
+        return MLC_ERR_OOM;
+    }
+}
+int mlc_executor_truncate_request(mlc_executor* e, uint32_t request_id, size_t tokens) {
+    if (!e || !e->paged) return MLC_ERR_INVALID_ARG;
+    return e->paged->truncate_request(request_id, tokens) ? MLC_OK : MLC_ERR_INVALID_ARG;
+}
+int mlc_executor_assign_beams(mlc_executor* e, const uint32_t* request_ids, const uint32_t* parents, size_t n) {
+    if (!e || !e->paged || (n && (!request_ids || !parents))) return MLC_ERR_INVALID_ARG;
+    try {
+        return e->paged->assign_beams(std::vector<uint32_t>(request_ids, request_ids + n), std::vector<uint32_t>(parents, parents + n))
+                   ? MLC_OK : MLC_ERR_INVALID_ARG;
+    } catch (const std::exception&) {
+        return MLC_ERR_OOM;
+    }
 }
 size_t mlc_executor_run_prefill(mlc_executor* e, uint32_t request_id, const uint64_t* tokens, size_t n,
                                 float* logits, size_t capacity) {

@@ -18,7 +18,7 @@ namespace mlcb {
 namespace {
 
 constexpr uint32_t kMaxPools = 128;      // per launch; a call with more takes several
-constexpr uint32_t kInlinePairs = 128;   // (source, destination) pairs that travel as kernel parameters
+constexpr uint32_t kInlinePairs = 64;    // (source, destination) pairs that travel as kernel parameters; longer lists cost less uploaded
 
 struct CopyParams {
     char* pools[kMaxPools];
@@ -106,13 +106,20 @@ int check_pools(mlc_ctx* ctx, void* const* pools, size_t n_pools, size_t P, size
     if (dtype_bytes != 2 && dtype_bytes != 4) return ctx->fail(MLC_ERR_INVALID_ARG, "dtype_bytes must be 2 or 4");
     if (P >= (size_t(1) << 32) || KVH >= (size_t(1) << 20) || D >= (size_t(1) << 20))
         return ctx->fail(MLC_ERR_UNSUPPORTED, "dimension too large");
-    std::vector<const void*> sorted(pools, pools + n_pools);
-    std::sort(sorted.begin(), sorted.end());
-    if (!sorted.front()) return ctx->fail(MLC_ERR_INVALID_ARG, "null pool");
-    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
-        return ctx->fail(MLC_ERR_INVALID_ARG, "a pool is named twice");
-    for (const void* p : sorted)
-        if (!aligned_to(p, dtype_bytes)) return ctx->fail(MLC_ERR_INVALID_ARG, "a pool is not aligned to its elements");
+    const void* few[256];
+    std::vector<const void*> many;
+    const void** sorted = few;
+    if (n_pools > 256) {
+        many.resize(n_pools);
+        sorted = many.data();
+    }
+    std::copy(pools, pools + n_pools, sorted);
+    std::sort(sorted, sorted + n_pools);
+    if (!sorted[0]) return ctx->fail(MLC_ERR_INVALID_ARG, "null pool");
+    for (size_t i = 0; i < n_pools; ++i) {
+        if (i && sorted[i] == sorted[i - 1]) return ctx->fail(MLC_ERR_INVALID_ARG, "a pool is named twice");
+        if (!aligned_to(sorted[i], dtype_bytes)) return ctx->fail(MLC_ERR_INVALID_ARG, "a pool is not aligned to its elements");
+    }
     return MLC_OK;
 }
 

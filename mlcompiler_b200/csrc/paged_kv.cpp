@@ -8,7 +8,7 @@
 namespace mlcb {
 namespace runtime {
 
-PagePool::PagePool(uint32_t capacity) : capacity_(capacity) {
+PagePool::PagePool(uint32_t capacity) : capacity_(capacity), owners_(capacity, 0) {
     stack_.resize(capacity);
     // id 0 ends on top, so a fresh pool allocates in ascending order (paged_kv.cpp:10-17)
     for (uint32_t i = 0; i < capacity; ++i) stack_[i] = capacity - 1 - i;
@@ -18,6 +18,7 @@ std::optional<uint32_t> PagePool::allocate() {
     if (stack_.empty()) return std::nullopt;
     const uint32_t id = stack_.back();
     stack_.pop_back();
+    owners_[id] = 1;
     ++in_use_;
     return id;
 }
@@ -25,6 +26,7 @@ std::optional<uint32_t> PagePool::allocate() {
 bool PagePool::allocate_n(size_t n, std::vector<uint32_t>& out) {
     if (n > stack_.size()) return false;
     out.insert(out.end(), stack_.rbegin(), stack_.rbegin() + static_cast<std::ptrdiff_t>(n));
+    for (size_t i = out.size() - n; i < out.size(); ++i) owners_[out[i]] = 1;
     stack_.resize(stack_.size() - n);
     in_use_ += n;
     return true;
@@ -32,8 +34,19 @@ bool PagePool::allocate_n(size_t n, std::vector<uint32_t>& out) {
 
 bool PagePool::release(uint32_t page_id) {
     if (page_id >= capacity_ || in_use_ == 0) return false;
+    if (owners_[page_id] > 1) {
+        --owners_[page_id];
+        return true;
+    }
+    owners_[page_id] = 0;
     stack_.push_back(page_id);
     --in_use_;
+    return true;
+}
+
+bool PagePool::share(uint32_t page_id) {
+    if (page_id >= capacity_ || owners_[page_id] == 0 || owners_[page_id] == UINT32_MAX) return false;
+    ++owners_[page_id];
     return true;
 }
 
@@ -44,8 +57,45 @@ bool RequestKVState::reserve(PagePool& pool, size_t target_tokens) {
     return pool.allocate_n(needed - page_table.size(), page_table);
 }
 
-std::optional<std::pair<uint32_t, uint32_t>> RequestKVState::extend_one_token(PagePool& pool) {
+bool RequestKVState::fork_from(const RequestKVState& parent, PagePool& pool) {
+    if (!page_table.empty() || &parent == this) return false;
+    std::vector<uint32_t> table;
+    table.reserve(parent.page_table.size());
+    for (uint32_t id : parent.page_table) {
+        if (!pool.share(id)) {
+            for (uint32_t taken : table) pool.release(taken);
+            return false;
+        }
+        table.push_back(id);
+    }
+    page_table = std::move(table);
+    page_size_tokens = parent.page_size_tokens;
+    tokens_in_last_page = parent.tokens_in_last_page;
+    return true;
+}
+
+bool RequestKVState::truncate(PagePool& pool, size_t tokens) {
+    if (page_size_tokens == 0 || tokens > total_tokens()) return false;
+    const size_t keep = (tokens + page_size_tokens - 1) / page_size_tokens;
+    while (page_table.size() > keep) {
+        pool.release(page_table.back());
+        page_table.pop_back();
+    }
+    tokens_in_last_page = keep ? static_cast<uint32_t>(tokens - (keep - 1) * page_size_tokens) : 0;
+    return true;
+}
+
+std::optional<std::pair<uint32_t, uint32_t>> RequestKVState::extend_one_token(PagePool& pool, PageCopies* copies) {
     if (page_size_tokens == 0) return std::nullopt;
+    if (!page_table.empty() && tokens_in_last_page < page_size_tokens && pool.owners(page_table.back()) > 1) {
+        if (!copies) return std::nullopt;
+        copies->reserve(copies->size() + 1);
+        const auto id = pool.allocate();
+        if (!id) return std::nullopt;  // table unchanged
+        copies->emplace_back(page_table.back(), *id);
+        pool.release(page_table.back());
+        page_table.back() = *id;
+    }
     if (page_table.empty() || tokens_in_last_page == page_size_tokens) {
         const auto id = pool.allocate();
         if (!id) return std::nullopt;  // table unchanged

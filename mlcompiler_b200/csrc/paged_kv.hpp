@@ -28,7 +28,12 @@ public:
     bool allocate_n(size_t n, std::vector<uint32_t>& out);
     // Returns false (and changes nothing) for an id outside the pool or with nothing in use;
     // the reference asserts in debug builds and is undefined in release builds.
+    // A page with several owners (see share) loses one of them and stays in use.
     bool release(uint32_t page_id);
+    // One more owner for a page in use (no counterpart in the reference, whose pages have one): a forked request shares
+    // its parent's pages until it writes. False for a page that is not in use.
+    bool share(uint32_t page_id);
+    uint32_t owners(uint32_t page_id) const { return page_id < capacity_ ? owners_[page_id] : 0; }
     uint32_t capacity() const { return capacity_; }
     size_t pages_in_use() const { return in_use_; }
     size_t pages_free() const { return stack_.size(); }
@@ -36,8 +41,12 @@ public:
 private:
     uint32_t capacity_;
     std::vector<uint32_t> stack_;  // top of the stack = next id handed out
+    std::vector<uint32_t> owners_; // per page id, 0 = free
     size_t in_use_ = 0;
 };
+
+// Pages to be copied before anything is written: (source, destination).
+using PageCopies = std::vector<std::pair<uint32_t, uint32_t>>;
 
 // One request's ordered page list and fill level (paged_kv.hpp:65-97). The page ids are
 // layer-agnostic: the same list indexes every layer's K and V pool.
@@ -52,7 +61,14 @@ struct RequestKVState {
                                   : (page_table.size() - 1) * static_cast<size_t>(page_size_tokens) + tokens_in_last_page;
     }
     bool reserve(PagePool& pool, size_t target_tokens);
-    std::optional<std::pair<uint32_t, uint32_t>> extend_one_token(PagePool& pool);
+    // The (page, slot) of one more token. A last page with room that other requests own too is replaced by a new one first,
+    // and the copy that the device then owes is appended to `copies`; without a list such a page makes the call fail.
+    std::optional<std::pair<uint32_t, uint32_t>> extend_one_token(PagePool& pool, PageCopies* copies = nullptr);
+    // This state becomes a second owner of every page of `parent`. False (and unchanged) if it has pages itself or a page
+    // cannot be shared.
+    bool fork_from(const RequestKVState& parent, PagePool& pool);
+    // Keeps the first `tokens` tokens and gives back the pages behind them. False if there are fewer.
+    bool truncate(PagePool& pool, size_t tokens);
     std::optional<std::pair<uint32_t, uint32_t>> locate(size_t pos) const;
     void release_all(PagePool& pool);
 };

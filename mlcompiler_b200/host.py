@@ -52,6 +52,16 @@ _PROTOTYPES = {
     "mlc_page_pool_allocate": (_i, [_vp, _u32p]),
     "mlc_page_pool_allocate_n": (_i, [_vp, _sz, _u32p]),
     "mlc_page_pool_release": (_i, [_vp, _u32]),
+    "mlc_page_pool_share": (_i, [_vp, _u32]),
+    "mlc_page_pool_owners": (_u32, [_vp, _u32]),
+    "mlc_kv_state_fork": (_i, [_vp, _vp, _vp]),
+    "mlc_kv_state_extend_one_token_owned": (_i, [_vp, _vp, _u32p, _u32p, _u32p, _u32p]),
+    "mlc_kv_state_truncate": (_i, [_vp, _vp, _sz]),
+    "mlc_executor_run_decode_beams": (_sz, [_vp, C.POINTER(RequestSlotC), _sz, _sz, _fp, C.POINTER(C.c_uint8), _sz, _u32,
+                                            _fp, _u32p, _u32p]),
+    "mlc_executor_fork_request": (_i, [_vp, _u32, _u32]),
+    "mlc_executor_truncate_request": (_i, [_vp, _u32, _sz]),
+    "mlc_executor_assign_beams": (_i, [_vp, _u32p, _u32p, _sz]),
     "mlc_page_pool_capacity": (_u32, [_vp]),
     "mlc_page_pool_in_use": (_sz, [_vp]),
     "mlc_page_pool_free": (_sz, [_vp]),
@@ -154,6 +164,13 @@ class PagePool:
     def release(self, page_id: int) -> bool:
         return bool(lib().mlc_page_pool_release(self._h, page_id))
 
+    def share(self, page_id: int) -> bool:
+        """One more owner for a page in use; release() takes one away."""
+        return bool(lib().mlc_page_pool_share(self._h, page_id))
+
+    def owners(self, page_id: int) -> int:
+        return lib().mlc_page_pool_owners(self._h, page_id)
+
     def capacity(self) -> int:
         return lib().mlc_page_pool_capacity(self._h)
 
@@ -180,6 +197,20 @@ class RequestKVState:
         p, s = _u32(0), _u32(0)
         ok = lib().mlc_kv_state_extend_one_token(self._h, pool._h, C.byref(p), C.byref(s))
         return (p.value, s.value) if ok else None
+
+    def extend_one_token_owned(self, pool: PagePool):
+        """(page, slot, None) or, where a shared page had to be replaced, (page, slot, (copy source, copy destination)): the copy
+        is owed before anything is written there. None when the pool is exhausted."""
+        p, s, a, b = _u32(0), _u32(0), _u32(0), _u32(0)
+        got = lib().mlc_kv_state_extend_one_token_owned(self._h, pool._h, C.byref(p), C.byref(s), C.byref(a), C.byref(b))
+        return (p.value, s.value, (a.value, b.value) if got == 2 else None) if got else None
+
+    def fork(self, parent: "RequestKVState", pool: PagePool) -> bool:
+        """This state, which has no pages, becomes a second owner of all of the parent's."""
+        return bool(lib().mlc_kv_state_fork(self._h, parent._h, pool._h))
+
+    def truncate(self, pool: PagePool, tokens: int) -> bool:
+        return bool(lib().mlc_kv_state_truncate(self._h, pool._h, tokens))
 
     def locate(self, pos: int):
         p, s = _u32(0), _u32(0)
@@ -452,6 +483,35 @@ class PagedAttentionExecutor(_ExecutorBase):
         if lib().mlc_executor_run_decode_greedy(self._h, arr, n, toks) != n or n == 0:
             return None
         return [None if int(t) == 2 ** 64 - 1 else int(t) for t in toks[:n]]
+
+    def run_decode_beams(self, slots, beams, cum_scores, n_select, finished=None, pad_token=0):
+        """A decode pass whose last step selects, per group of `beams` slots, the n_select best continuations on the device:
+        (scores, parents, tokens), each [groups, n_select], or None when the executor cannot do it or the pass failed."""
+        n = len(slots)
+        arr = (RequestSlotC * max(n, 1))(*[RequestSlotC(*s) for s in slots])
+        cum = np.ascontiguousarray(cum_scores, np.float32)
+        done = np.ascontiguousarray(finished, np.uint8) if finished is not None else None
+        if cum.size != n or (done is not None and done.size != n) or not beams or n % beams:
+            return None
+        shape = (n // beams, n_select)
+        scores, parents, tokens = np.zeros(shape, np.float32), np.zeros(shape, np.uint32), np.zeros(shape, np.uint32)
+        got = lib().mlc_executor_run_decode_beams(
+            self._h, arr, n, beams, cum.ctypes.data_as(_fp), done.ctypes.data_as(C.POINTER(C.c_uint8)) if done is not None else None,
+            n_select, pad_token, scores.ctypes.data_as(_fp), parents.ctypes.data_as(_u32p), tokens.ctypes.data_as(_u32p))
+        return (scores, parents, tokens) if got == n and n else None
+
+    def fork_request(self, parent_id, child_id) -> bool:
+        return lib().mlc_executor_fork_request(self._h, parent_id, child_id) == 0
+
+    def truncate_request(self, request_id, tokens) -> bool:
+        return lib().mlc_executor_truncate_request(self._h, request_id, tokens) == 0
+
+    def assign_beams(self, request_ids, parents) -> bool:
+        """request_ids[i] continues from where request_ids[parents[i]] is now, for all i at once."""
+        ids, par = np.ascontiguousarray(request_ids, np.uint32), np.ascontiguousarray(parents, np.uint32)
+        if ids.size != par.size:
+            return False
+        return lib().mlc_executor_assign_beams(self._h, ids.ctypes.data_as(_u32p), par.ctypes.data_as(_u32p), ids.size) == 0
 
     def run_prefill(self, request_id, tokens):
         toks = (C.c_uint64 * max(len(tokens), 1))(*tokens)

@@ -23,6 +23,7 @@ struct mlc_tree_plan {
     uint8_t* dev = nullptr;
     size_t cap = 0;
     cudaEvent_t uploaded = nullptr;
+    bool ready = false;   // the image of `view` is on its way to the device
     mutable bool captured = false;
 };
 
@@ -232,7 +233,7 @@ int fill_plan(mlc_ctx* ctx, mlc_tree_plan& p, TreeShape s, const TreeTables& t, 
         }
         MLCB_CUDA(ctx, cudaStreamSynchronize(ctx->stream));   // kernels that read the old image
         release_buffers(p);
-        p.shape.tokens = 0;   // nothing to launch until the new image is on its way
+        p.ready = false;      // until the new image is on its way
         p.host = h;
         p.dev = d;
         p.cap = want;
@@ -246,6 +247,7 @@ int fill_plan(mlc_ctx* ctx, mlc_tree_plan& p, TreeShape s, const TreeTables& t, 
     MLCB_CUDA(ctx, cudaEventRecord(p.uploaded, ctx->stream));
     p.shape = s;
     p.view = view_of(p.dev, l, w);
+    p.ready = true;
     return MLC_OK;
 }
 
@@ -326,6 +328,7 @@ int mlc_encode_paged_tree_attention_planned(mlc_ctx* ctx, const mlc_tree_plan* p
     if (!ctx || !plan) return MLC_ERR_INVALID_ARG;
     if (plan->ctx != ctx) return ctx->fail(MLC_ERR_INVALID_ARG, "the plan belongs to another context");
     if (!ctx->pass_open) return ctx->fail(MLC_ERR_NO_OPEN_PASS, "encode without an open pass");
+    if (!plan->ready) return ctx->fail(MLC_ERR_INVALID_ARG, "the plan lost its tables in a failed update");
     const TreeArgs a{q, k_pages, v_pages, o, scale, q_dtype, o_dtype};
     const int st = check_call(ctx, a);
     if (st != MLC_OK) return st;

@@ -15,7 +15,8 @@
 // that do see them.
 //
 // fp32 queries or outputs (EXACT): an fp16 operand carries 11 bits, so Q (scaled by a power of two per row) and P enter as
-// two fp16 halves, two products each: 22 bits of each, K and V are fp16 as they are.
+// two fp16 halves, two products each: 22 bits of each, K and V are fp16 as they are. The products of a tile are added to
+// those before it outside the tensor core.
 //
 // What bounds it: the cache is read once, 4 * rows flop per byte - memory up to about 128 rows, the exponentials and the
 // tensor core's issue above. The cache tiles of all (request, KV head, row tile) units are dealt evenly to a resident
@@ -37,9 +38,6 @@ namespace {
 
 constexpr uint32_t kSlabQ = kTreeRows * 128;   // 64 halfs of every query row
 constexpr uint32_t kSlabKV = kTreeTile * 128;  // 64 halfs of every token of a tile
-constexpr uint32_t kTmemCols = 256;            // O: up to 128 columns, S: 2 x 64; D = 64: Q behind O
-constexpr uint32_t kTmemS = 128;
-constexpr uint32_t kTmemQ = 64;
 constexpr uint32_t kThreads = 224;
 constexpr uint32_t kStageBytes = 32 * 128;     // per softmax warp: 128 bytes of each of its rows, on the way in or out
 
@@ -48,12 +46,15 @@ struct Config {
     static constexpr uint32_t slabs = D / 64;
     // Q as an operand in tensor memory where there is room beside O and S: read from shared memory, its 128 rows cost
     // every product twice what the 64 rows of K do
-    static constexpr bool q_tmem = D == 64;
+    static constexpr bool q_tmem = D == 64 && !EXACT;
+    // Columns of tensor memory: O, then Q or (EXACT) the sum over the tiles before, then two S buffers
+    static constexpr uint32_t tmem_q = D, tmem_sum = D, tmem_s = D == 128 && EXACT ? 256 : 128;
+    static constexpr uint32_t tmem_cols = D == 128 && EXACT ? 512 : 256;
     static constexpr uint32_t q_bytes = q_tmem ? 0 : slabs * kSlabQ * (EXACT ? 2 : 1);
     static constexpr uint32_t kv_bytes = slabs * kSlabKV;   // one tile of K, or of V
     // two CTAs per SM share 226 KB; with D = 128 the two halves of Q leave room for one CTA only
     static constexpr uint32_t ctas = EXACT && D == 128 ? 1 : 2;
-    static constexpr uint32_t stages = D == 64 ? 6 : EXACT ? 4 : 2;
+    static constexpr uint32_t stages = EXACT ? 4 : D == 64 ? 6 : 2;
     static constexpr uint32_t tile_bytes = q_bytes + stages * 2 * kv_bytes;
     static constexpr uint32_t smem_bytes = tile_bytes + 4 * kStageBytes;   // and the barriers behind that
 };
@@ -130,10 +131,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
-}
-__device__ __forceinline__ void tmem_st4(uint32_t taddr, const uint32_t (&r)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -282,16 +279,10 @@ __device__ __forceinline__ float load_queries(uint32_t sQ, uint32_t tQ, uint32_t
                     lo[i] = pack(a - back.x, b - back.y);
                 }
                 const uint32_t at = k * per_block + c;
-                if constexpr (TMEM) {
-                    tmem_st4(tQ + 4 * at, hi);
-                    tmem_st4(tQ + D / 2 + 4 * at, lo);
-                } else {
-                    to_shared(0, at, hi);
-                    to_shared(1, at, lo);
-                }
+                to_shared(0, at, hi);
+                to_shared(1, at, lo);
             }
         }
-        if constexpr (TMEM) tmem_wait_st();
         return down;
     }
 }
@@ -327,7 +318,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
         bars.not_finite = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 4) tc::tmem_alloc(smem_u32(&bars.tmem_slot), kTmemCols);
+    if (warp == 4) tc::tmem_alloc(smem_u32(&bars.tmem_slot), C::tmem_cols);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
@@ -403,20 +394,22 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
         const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0), sQ_u = __shfl_sync(0xffffffffu, sQ, 0);
         const uint32_t sKV_u = sQ_u + C::q_bytes;
         auto issue_qk = [&](uint32_t g) {
-            const uint32_t s = g % STAGES, sK = sKV_u + s * 2 * C::kv_bytes, d = tmem_u + kTmemS + (g & 1u) * kTreeTile;
+            const uint32_t s = g % STAGES, sK = sKV_u + s * 2 * C::kv_bytes, d = tmem_u + C::tmem_s + (g & 1u) * kTreeTile;
             if (tc::elect_one()) {
 #pragma unroll
-                for (uint32_t half = 0; half < (EXACT ? 2u : 1u); ++half)
+                for (uint32_t h = 0; h < (EXACT ? 2u : 1u); ++h) {   // the low halves first: fewer roundings at full magnitude
+                    const uint32_t half = EXACT ? 1 - h : 0;
 #pragma unroll
                     for (uint32_t k = 0; k < D / 16; ++k) {
                         const uint32_t b = sK + (k >> 2) * kSlabKV + (k & 3) * 32;
                         if constexpr (C::q_tmem) {
-                            mma_f16_ts(d, tmem_u + kTmemQ + half * 32 + k * 8, desc_k | (b >> 4), idesc_qk, half + k > 0);
+                            mma_f16_ts(d, tmem_u + C::tmem_q + k * 8, desc_k | (b >> 4), idesc_qk, k > 0);
                         } else {
                             const uint32_t a = sQ_u + (half * C::slabs + (k >> 2)) * kSlabQ + (k & 3) * 32;
-                            tc::mma_f16(d, desc_k | (a >> 4), desc_k | (b >> 4), idesc_qk, half + k > 0);
+                            tc::mma_f16(d, desc_k | (a >> 4), desc_k | (b >> 4), idesc_qk, h + k > 0);
                         }
                     }
+                }
                 tc::commit(smem_u32(&bars.k_empty[s]));
                 tc::commit(smem_u32(&bars.s_full[g & 1u]));
             }
@@ -454,14 +447,14 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 }
                 tc::fence_after();
                 const uint32_t sV = sKV_u + s * 2 * C::kv_bytes + C::kv_bytes;
-                const uint32_t P = tmem_u + kTmemS + (g & 1u) * kTreeTile;
+                const uint32_t P = tmem_u + C::tmem_s + (g & 1u) * kTreeTile;
                 if (tc::elect_one()) {
 #pragma unroll
-                    for (uint32_t half = 0; half < (EXACT ? 2u : 1u); ++half)
+                    for (uint32_t h = 0; h < (EXACT ? 2u : 1u); ++h)
 #pragma unroll
                         for (uint32_t k = 0; k < kTreeTile / 16; ++k)   // 16 tokens per step: 8 columns of P, 16 rows of V
-                            mma_f16_ts(tmem_u, P + half * 32 + k * 8, desc_v | ((sV + k * 16 * 128) >> 4), idesc_pv,
-                                       j > 0 || half + k > 0);
+                            mma_f16_ts(tmem_u, P + (EXACT ? 1 - h : 0) * 32 + k * 8, desc_v | ((sV + k * 16 * 128) >> 4), idesc_pv,
+                                       (j > 0 && !EXACT) || h + k > 0);
                     tc::commit(smem_u32(&bars.v_empty[s]));
                     tc::commit(smem_u32(&bars.pv_done));
                 }
@@ -484,7 +477,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
         auto put_query = [&](const TreePiece& pc) {
             const uint32_t r = pc.row_begin + row;
             const size_t elem = (static_cast<size_t>(pc.token0 + r / prm.G) * prm.H + pc.kv_head * prm.G + r % prm.G) * D;
-            row_down = load_queries<D, EXACT>(sQ, tmem + lane_base + kTmemQ, stage, row, prm.q, prm.q_f32, row < pc.n_rows, elem);
+            row_down = load_queries<D, EXACT>(sQ, tmem + lane_base + C::tmem_q, stage, row, prm.q, prm.q_f32, row < pc.n_rows, elem);
             if constexpr (C::q_tmem) tc::fence_before();
             else tc::fence_proxy_async_smem();
             tc::mbar_arrive(smem_u32(&bars.q_full));
@@ -505,8 +498,9 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 if (!ok) break;
                 tc::fence_after();
                 if (busy) {
-                    const uint32_t tS = tmem + lane_base + kTmemS + (g & 1u) * kTreeTile;
+                    const uint32_t tS = tmem + lane_base + C::tmem_s + (g & 1u) * kTreeTile;
                     uint32_t hi[32], lo[EXACT ? 32 : 1];
+                    float alpha = 1.0f;
                     // First with the reference maximum as it is, without looking for the tile's: every weight is below the
                     // row's sum over the tile, and while that is below 2^15 the weights fit fp16. Where some row's sum is not
                     // (or is NaN), and on a run's first tile, the tile is done (again) with a new reference.
@@ -538,7 +532,6 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                                 if (!((see_hi >> c) & 1u)) s[32 + c] = 0xff800000u;
                             }
                         }
-                        float alpha = 1.0f;
                         if (moved) {
                             float top = m_ref;   // fmaxf passes over NaN
 #pragma unroll
@@ -570,7 +563,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                         if (!moved) {
                             // (a reference of -inf is none)
                             if (__any_sync(0xffffffffu, !(sum < 32768.0f) || m_ref == -INFINITY)) continue;
-                        } else if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                        } else if (!EXACT && j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
                             where = 0x21;
                             ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
                             if (!ok) break;
@@ -591,7 +584,31 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                     if (!ok) break;
                     // P over this tile's scores (own lane, already read): the halves in 32 columns each
                     tmem_st32(tS, hi);
-                    if constexpr (EXACT) tmem_st32(tS + 32, lo);
+                    if constexpr (EXACT) {
+                        tmem_st32(tS + 32, lo);
+                        // The tensor core drops what falls below an accumulator's last bit, always towards zero: over a few
+                        // hundred tokens that is 1e-6 of the result. So P.V of a tile starts from zero, and the tiles are added
+                        // here, rounding to nearest.
+                        if (j > 0) {
+                            where = 0x26;
+                            ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);
+                            if (!ok) break;
+                            tc::fence_after();
+#pragma unroll 1
+                            for (int c0 = 0; c0 < D; c0 += 32) {
+                                uint32_t o[32], sum[32];
+                                tc::tmem_ld32(tmem + lane_base + c0, o);
+                                if (j > 1) tc::tmem_ld32(tmem + lane_base + C::tmem_sum + c0, sum);
+                                tc::tmem_wait_ld();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) {
+                                    const float before = j > 1 ? __uint_as_float(sum[i]) : 0.f;
+                                    sum[i] = __float_as_uint((before + __uint_as_float(o[i])) * alpha);
+                                }
+                                tmem_st32(tmem + lane_base + C::tmem_sum + c0, sum);
+                            }
+                        }
+                    }
                     tmem_wait_st();
                 }
                 if (kv0 + kTreeTile > p.prefix) {
@@ -679,6 +696,13 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                         uint32_t o[32];
                         tc::tmem_ld32(tmem + lane_base + c0 + 32 * half, o);
                         tc::tmem_wait_ld();
+                        if (EXACT && done.n_tiles > 1) {
+                            uint32_t sum[32];
+                            tc::tmem_ld32(tmem + lane_base + C::tmem_sum + c0 + 32 * half, sum);
+                            tc::tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(sum[i]) + __uint_as_float(o[i]));
+                        }
                         if (repair && mine) put_back(c0 + 32 * half, o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
@@ -699,7 +723,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    if (warp == 4) tc::tmem_dealloc(tmem, kTmemCols);
+    if (warp == 4) tc::tmem_dealloc(tmem, C::tmem_cols);
 }
 
 // O of the rows whose run was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. WARPS warps per row

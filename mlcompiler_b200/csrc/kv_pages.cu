@@ -104,7 +104,7 @@ int check_pools(mlc_ctx* ctx, void* const* pools, size_t n_pools, size_t P, size
     if (!pools) return ctx->fail(MLC_ERR_INVALID_ARG, "null argument");
     if (n_pools == 0 || P == 0 || KVH == 0 || D == 0) return ctx->fail(MLC_ERR_INVALID_ARG, "zero dimension");
     if (dtype_bytes != 2 && dtype_bytes != 4) return ctx->fail(MLC_ERR_INVALID_ARG, "dtype_bytes must be 2 or 4");
-    if (P >= (size_t(1) << 32) || KVH >= (size_t(1) << 20) || D >= (size_t(1) << 20))
+    if (KVH >= (size_t(1) << 20) || D >= (size_t(1) << 20) || P >= (size_t(1) << 40) / (KVH * D))
         return ctx->fail(MLC_ERR_UNSUPPORTED, "dimension too large");
     const void* few[256];
     std::vector<const void*> many;

@@ -52,14 +52,25 @@ struct TreeWork {
     uint32_t n_slots = 0, slot_rows = 0, max_parts = 0;
 };
 
-struct TreeView {   // device addresses inside one image
-    const uint32_t *pt_flat = nullptr, *pt_off = nullptr, *prefix = nullptr, *draft = nullptr, *mask = nullptr;
-    const uint32_t *token0 = nullptr;     // first drafted token of a request in q / o, [batch + 1]
-    const uint32_t *token_req = nullptr;  // request of a drafted token
+struct TreeWorkView {   // a work list on the device
     const TreePiece* pieces = nullptr;
     const TreeSplit* splits = nullptr;
     const uint32_t* row_split = nullptr;
     uint32_t n_cta = 0, n_slots = 0, slot_rows = 0, merge_rows = 0, max_parts = 0;
+};
+
+// The tensor-core kernel runs two CTAs per SM, with fp32 queries or outputs and head_dim 128 one: a call with its tables in a
+// plan may be either, so head_dim 128 has two lists.
+static constexpr uint32_t kTreeLists = 2;   // [0]: two CTAs per SM, [1]: one
+struct TreeWorks {
+    TreeWork list[kTreeLists];
+};
+
+struct TreeView {   // device addresses inside one image
+    const uint32_t *pt_flat = nullptr, *pt_off = nullptr, *prefix = nullptr, *draft = nullptr, *mask = nullptr;
+    const uint32_t *token0 = nullptr;     // first drafted token of a request in q / o, [batch + 1]
+    const uint32_t* token_req = nullptr;  // request of a drafted token
+    TreeWorkView work[kTreeLists];
 };
 
 struct TreeArgs {
@@ -75,7 +86,6 @@ struct TreeArgs {
 // known size; and these buffers.
 bool tree_tcgen05_shape(const TreeShape& s);
 bool tree_tcgen05_buffers(const TreeArgs& a);
-static constexpr uint32_t kTreeCtasPerSm = 2;
 // Cuts the units of a call into pieces for `max_ctas` CTAs (host arithmetic only).
 void tree_work_list(const TreeShape& s, const TreeTables& t, uint32_t max_ctas, TreeWork* out);
 // Device scratch for the partials of cut units.

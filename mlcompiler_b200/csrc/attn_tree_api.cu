@@ -33,10 +33,11 @@ size_t align16(size_t v) { return (v + 15) / 16 * 16; }
 
 // Offsets of an image's parts.
 struct TreeLayout {
-    size_t flat, off, prefix, draft, token0, token_req, mask, pieces, splits, row_split, total;
+    size_t flat, off, prefix, draft, token0, token_req, mask, total;
+    size_t pieces[kTreeLists], splits[kTreeLists], row_split[kTreeLists];
 };
 
-TreeLayout layout_of(const TreeShape& s, const TreeWork& w) {
+TreeLayout layout_of(const TreeShape& s, const TreeWorks& w) {
     TreeLayout l{};
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -44,9 +45,11 @@ TreeLayout layout_of(const TreeShape& s, const TreeWork& w) {
         at = align16(at + bytes);
         return here;
     };
-    l.pieces = take(w.pieces.size() * sizeof(TreePiece));
-    l.splits = take(w.splits.size() * sizeof(TreeSplit));
-    l.row_split = take(w.row_split.size() * 4);
+    for (uint32_t i = 0; i < kTreeLists; ++i) {
+        l.pieces[i] = take(w.list[i].pieces.size() * sizeof(TreePiece));
+        l.splits[i] = take(w.list[i].splits.size() * sizeof(TreeSplit));
+        l.row_split[i] = take(w.list[i].row_split.size() * 4);
+    }
     l.flat = take(s.n_flat * 4);
     l.off = take((s.batch + 1) * 4);
     l.prefix = take(s.batch * 4);
@@ -62,10 +65,12 @@ void put(uint8_t* at, const void* src, size_t bytes) {
     if (bytes) std::memcpy(at, src, bytes);
 }
 
-void fill_image(uint8_t* h, const TreeLayout& l, const TreeShape& s, const TreeTables& t, const TreeWork& w) {
-    put(h + l.pieces, w.pieces.data(), w.pieces.size() * sizeof(TreePiece));
-    put(h + l.splits, w.splits.data(), w.splits.size() * sizeof(TreeSplit));
-    put(h + l.row_split, w.row_split.data(), w.row_split.size() * 4);
+void fill_image(uint8_t* h, const TreeLayout& l, const TreeShape& s, const TreeTables& t, const TreeWorks& w) {
+    for (uint32_t i = 0; i < kTreeLists; ++i) {
+        put(h + l.pieces[i], w.list[i].pieces.data(), w.list[i].pieces.size() * sizeof(TreePiece));
+        put(h + l.splits[i], w.list[i].splits.data(), w.list[i].splits.size() * sizeof(TreeSplit));
+        put(h + l.row_split[i], w.list[i].row_split.data(), w.list[i].row_split.size() * 4);
+    }
     put(h + l.flat, t.pt_flat, s.n_flat * 4);
     put(h + l.off, t.pt_off, (s.batch + 1) * 4);
     put(h + l.prefix, t.prefix, s.batch * 4);
@@ -81,7 +86,7 @@ void fill_image(uint8_t* h, const TreeLayout& l, const TreeShape& s, const TreeT
     put(h + l.mask, t.mask, s.tokens * s.mask_words * 4);
 }
 
-TreeView view_of(const uint8_t* dev, const TreeLayout& l, const TreeWork& w) {
+TreeView view_of(const uint8_t* dev, const TreeLayout& l, const TreeWorks& w) {
     TreeView v;
     auto words = [&](size_t at) { return reinterpret_cast<const uint32_t*>(dev + at); };
     v.pt_flat = words(l.flat);
@@ -91,14 +96,18 @@ TreeView view_of(const uint8_t* dev, const TreeLayout& l, const TreeWork& w) {
     v.token0 = words(l.token0);
     v.token_req = words(l.token_req);
     v.mask = words(l.mask);
-    v.pieces = reinterpret_cast<const TreePiece*>(dev + l.pieces);
-    v.splits = reinterpret_cast<const TreeSplit*>(dev + l.splits);
-    v.row_split = words(l.row_split);
-    v.n_cta = w.n_cta;
-    v.n_slots = w.n_slots;
-    v.slot_rows = w.slot_rows;
-    v.max_parts = w.max_parts;
-    v.merge_rows = static_cast<uint32_t>(w.row_split.size());
+    for (uint32_t i = 0; i < kTreeLists; ++i) {
+        const TreeWork& list = w.list[i];
+        TreeWorkView& out = v.work[i];
+        out.pieces = reinterpret_cast<const TreePiece*>(dev + l.pieces[i]);
+        out.splits = reinterpret_cast<const TreeSplit*>(dev + l.splits[i]);
+        out.row_split = words(l.row_split[i]);
+        out.n_cta = list.n_cta;
+        out.n_slots = list.n_slots;
+        out.slot_rows = list.slot_rows;
+        out.max_parts = list.max_parts;
+        out.merge_rows = static_cast<uint32_t>(list.row_split.size());
+    }
     return v;
 }
 
@@ -152,7 +161,7 @@ int check_call(mlc_ctx* ctx, const TreeArgs& a) {
 int launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, TreeArgs a) {
     if (s.tokens == 0) return MLC_OK;
     if (!(a.scale > 0.f)) a.scale = 1.0f / std::sqrt(static_cast<float>(s.D));
-    if (v.n_cta && !ctx->force_general && tree_tcgen05_buffers(a)) {
+    if (v.work[0].n_cta && !ctx->force_general && tree_tcgen05_buffers(a)) {
         ctx->last_attention_kernel = 4;
         return launch_tree_tcgen05(ctx, s, v, a);
     }
@@ -160,11 +169,15 @@ int launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, TreeArgs a) {
     return launch_tree_general(ctx, s, v, a);
 }
 
-// The work list of the tensor-core kernel, and room for its partials.
-int prepare_work(mlc_ctx* ctx, const TreeShape& s, const TreeTables& t, TreeWork* w) {
+// The work lists of the tensor-core kernel, and room for their partials.
+int prepare_work(mlc_ctx* ctx, const TreeShape& s, const TreeTables& t, TreeWorks* w) {
     if (!tree_tcgen05_shape(s)) return MLC_OK;
-    tree_work_list(s, t, static_cast<uint32_t>(ctx->sm_count) * kTreeCtasPerSm, w);
-    return ensure_op_scratch(ctx, ctx->tree_scratch, tree_scratch_bytes(s, w->n_slots, w->slot_rows), "tree attention scratch");
+    size_t bytes = 0;
+    for (uint32_t i = 0; i < (s.D == 128 ? kTreeLists : 1u); ++i) {
+        tree_work_list(s, t, static_cast<uint32_t>(ctx->sm_count) * (i ? 1u : 2u), &w->list[i]);
+        bytes = std::max(bytes, tree_scratch_bytes(s, w->list[i].n_slots, w->list[i].slot_rows));
+    }
+    return ensure_op_scratch(ctx, ctx->tree_scratch, bytes, "tree attention scratch");
 }
 
 // One call with host tables: the image goes through the context's staging area.
@@ -179,7 +192,7 @@ int tree_impl(mlc_ctx* ctx, bool sync, const TreeArgs& a, TreeShape s, const Tre
     if (ctx->capturing) return ctx->fail(MLC_ERR_UNSUPPORTED, "host tables inside a graph capture: use a plan");
     if (s.tokens == 0) return MLC_OK;
     DeviceGuard guard(ctx->device);
-    TreeWork w;
+    TreeWorks w;
     if ((st = prepare_work(ctx, s, t, &w)) != MLC_OK) return st;
     const TreeLayout l = layout_of(s, w);
     void *h = nullptr, *d = nullptr;
@@ -215,7 +228,7 @@ int fill_plan(mlc_ctx* ctx, mlc_tree_plan& p, TreeShape s, const TreeTables& t, 
     if (st != MLC_OK) return ctx->fail(st, "%s", why.c_str());
     if (ctx->capturing) return ctx->fail(MLC_ERR_UNSUPPORTED, "new tables inside a graph capture: create the plan before capturing");
     DeviceGuard guard(ctx->device);
-    TreeWork w;
+    TreeWorks w;
     if ((st = prepare_work(ctx, s, t, &w)) != MLC_OK) return st;
     const TreeLayout l = layout_of(s, w);
     if (!p.uploaded) MLCB_CUDA(ctx, cudaEventCreateWithFlags(&p.uploaded, cudaEventDisableTiming));

@@ -165,17 +165,19 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) { return ((w & 0x7C00
 // its own row. 16-byte chunk c of row r sits at r * 128 + ((c ^ r) & 7) * 16.
 __device__ __forceinline__ uint32_t staged(uint32_t stage, uint32_t r, uint32_t c) { return stage + r * 128 + (((c ^ r) & 7u) << 4); }
 
-// 128 bytes, from byte `offset` of this lane's row on (rows of invalid lanes: zeros), to shared memory.
-__device__ __forceinline__ void stage_in(uint32_t stage, uint32_t lane, const char* row, bool valid, uint32_t offset) {
+// 128 bytes, from byte `offset` of this lane's row on (rows of invalid lanes: zeros), into registers: lane i holds chunk i % 8 of
+// row i / 8 and of every fourth row behind it.
+__device__ __forceinline__ void stage_load(uint4 (&v)[8], uint32_t lane, const char* row, bool valid, uint32_t offset) {
     const uint32_t rows = __ballot_sync(0xffffffffu, valid);
     const uint64_t mine = reinterpret_cast<uint64_t>(row + offset);
-    uint4 v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t r = 4 * i + (lane >> 3);
         const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, mine, r));
         v[i] = (rows >> r) & 1u ? __ldg(reinterpret_cast<const uint4*>(src) + (lane & 7u)) : make_uint4(0, 0, 0, 0);
     }
+}
+__device__ __forceinline__ void stage_put(uint32_t stage, uint32_t lane, const uint4 (&v)[8]) {
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 8; ++i) st_shared16(staged(stage, 4 * i + (lane >> 3), lane & 7u), v[i]);
@@ -198,6 +200,11 @@ __device__ __forceinline__ void stage_out(uint32_t stage, uint32_t lane, char* r
     }
 }
 
+template <int N>
+struct Blocks {
+    static constexpr int value = N;
+};
+
 // Puts the warp's query rows (zeros for invalid lanes) into the operand tile(s), in shared memory (swizzled) or in tensor
 // memory; returns what the lane's scores have to be multiplied with to undo its row's scaling.
 template <int D, bool EXACT>
@@ -211,14 +218,17 @@ __device__ __forceinline__ float load_queries(uint32_t sQ, uint32_t tQ, uint32_t
     };
     const char* src = static_cast<const char*>(q) + elem * (q_f32 ? 4 : 2);
     if constexpr (!EXACT) {
+        uint4 v[D / 64][8];
 #pragma unroll
-        for (int block = 0; block < D / 64; ++block) {   // 64 halfs
-            stage_in(stage, lane, src, valid, block * 128);
+        for (int block = 0; block < D / 64; ++block) stage_load(v[block], lane, src, valid, block * 128);   // 64 halfs
+#pragma unroll
+        for (int block = 0; block < D / 64; ++block) {
+            stage_put(stage, lane, v[block]);
             uint32_t w[32];
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
-                const uint4 v = ld_shared16(staged(stage, lane, c));
-                w[4 * c] = v.x; w[4 * c + 1] = v.y; w[4 * c + 2] = v.z; w[4 * c + 3] = v.w;
+                const uint4 x = ld_shared16(staged(stage, lane, c));
+                w[4 * c] = x.x; w[4 * c + 1] = x.y; w[4 * c + 2] = x.z; w[4 * c + 3] = x.w;
             }
             if constexpr (TMEM) {
                 tmem_st32(tQ, w);
@@ -230,60 +240,56 @@ __device__ __forceinline__ float load_queries(uint32_t sQ, uint32_t tQ, uint32_t
         if constexpr (TMEM) tmem_wait_st();
         return 1.0f;
     } else {
-        // 8 columns of the lane's row out of the block of 32 (fp32) or 64 (fp16) that is staged
-        auto read8 = [&](uint32_t c, float (&x)[8]) {
-            if (q_f32) {
-                const uint4 a = ld_shared16(staged(stage, lane, 2 * c)), b = ld_shared16(staged(stage, lane, 2 * c + 1));
-                const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        // All of the row is under way at once, then each lane finds its own in shared memory and keeps it.
+        float scale_down = 1.0f;
+        auto run = [&](auto n_blocks, auto column) {
+            constexpr int N = decltype(n_blocks)::value;
+            uint32_t w[N][32];
+            {
+                uint4 v[N][8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
-            } else {
-                const uint4 a = ld_shared16(staged(stage, lane, c));
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+                for (int i = 0; i < N; ++i) stage_load(v[i], lane, src, valid, i * 128);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                    x[2 * i] = f.x; x[2 * i + 1] = f.y;
+                for (int i = 0; i < N; ++i) {
+                    stage_put(stage, lane, v[i]);
+#pragma unroll
+                    for (int c = 0; c < 8; ++c) {
+                        const uint4 x = ld_shared16(staged(stage, lane, c));
+                        w[i][4 * c] = x.x; w[i][4 * c + 1] = x.y; w[i][4 * c + 2] = x.z; w[i][4 * c + 3] = x.w;
+                    }
                 }
             }
-        };
-        const uint32_t per_block = q_f32 ? 4 : 8, blocks = D / 8 / per_block;   // groups of 8 columns
-        float top = 0.f;
-        for (uint32_t k = 0; k < blocks; ++k) {
-            stage_in(stage, lane, src, valid, k * 128);
-#pragma unroll 2
-            for (uint32_t c = 0; c < per_block; ++c) {
-                float x[8];
-                read8(c, x);
+            float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
-            }
-        }
-        // largest magnitude to [2^7, 2^8): well inside fp16, and the low halves stay clear of its subnormals
-        int shift = 0;
-        if (top > 0.f && top < INFINITY) shift = max(-120, min(120, 7 - ilogbf(top)));
-        const float up = __int_as_float((127 + shift) << 23), down = __int_as_float((127 - shift) << 23);
-        for (uint32_t k = 0; k < blocks; ++k) {
-            stage_in(stage, lane, src, valid, k * 128);
-#pragma unroll 2
-            for (uint32_t c = 0; c < per_block; ++c) {
-                float x[8];
-                read8(c, x);
+            for (int d = 0; d < D; ++d) top = fmaxf(top, fabsf(column(w, d)));
+            // largest magnitude to [2^7, 2^8): well inside fp16, and the low halves stay clear of its subnormals
+            int shift = 0;
+            if (top > 0.f && top < INFINITY) shift = max(-120, min(120, 7 - ilogbf(top)));
+            const float up = __int_as_float((127 + shift) << 23);
+            scale_down = __int_as_float((127 - shift) << 23);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float a = x[2 * i] * up, b = x[2 * i + 1] * up;
+                    const float a = column(w, 8 * c + 2 * i) * up, b = column(w, 8 * c + 2 * i + 1) * up;
                     const __half2 h = __floats2half2_rn(a, b);
                     const float2 back = __half22float2(h);
                     hi[i] = *reinterpret_cast<const uint32_t*>(&h);
                     lo[i] = pack(a - back.x, b - back.y);
                 }
-                const uint32_t at = k * per_block + c;
-                to_shared(0, at, hi);
-                to_shared(1, at, lo);
+                to_shared(0, c, hi);
+                to_shared(1, c, lo);
             }
-        }
-        return down;
+        };
+        if (q_f32)
+            run(Blocks<D / 32>(), [](const auto& w, int d) { return __uint_as_float(w[d / 32][d % 32]); });
+        else
+            run(Blocks<D / 64>(), [](const auto& w, int d) {
+                const uint32_t x = w[d / 64][d % 64 / 2];
+                return __half2float(__ushort_as_half(static_cast<unsigned short>(d % 2 ? x >> 16 : x & 0xFFFFu)));
+            });
+        return scale_down;
     }
 }
 
@@ -809,7 +815,7 @@ int pool_map(mlc_ctx* ctx, CUtensorMap* out, const void* pool, const TreeShape& 
 }
 
 template <int D, typename OT>
-cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const float* part_o, const float2* part_ml, void* o) {
+cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeWorkView& v, const float* part_o, const float2* part_ml, void* o) {
     // many parts a row: four warps share it
     const bool wide = v.max_parts > 8;
     auto kernel = wide ? tree_merge_kernel<D, 4, OT> : tree_merge_kernel<D, 1, OT>;
@@ -822,6 +828,8 @@ template <int D, bool EXACT>
 int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a) {
     using C = Config<D, EXACT>;
     constexpr size_t smem = C::smem_bytes + sizeof(Bars<C::stages>);
+    static_assert((smem + 1024) * C::ctas <= 228 * 1024, "CTAs per SM");
+    const TreeWorkView& w = v.work[C::ctas == 1 ? 1 : 0];
     const uint32_t box_rows = static_cast<uint32_t>(s.P < kTreeTile ? s.P : kTreeTile);
     CUtensorMap mk, mv;
     int st = pool_map(ctx, &mk, a.k_pages, s, box_rows);
@@ -837,11 +845,11 @@ int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs
     p.q = a.q;
     p.v_pages = static_cast<const __half*>(a.v_pages);
     p.o = a.o;
-    if (v.n_slots) {
+    if (w.n_slots) {
         p.part_o = static_cast<float*>(ctx->tree_scratch.dev);
-        p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(v.n_slots) * v.slot_rows * D);
+        p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(w.n_slots) * w.slot_rows * D);
     }
-    p.pieces = v.pieces;
+    p.pieces = w.pieces;
     p.pt_flat = v.pt_flat;
     p.mask = v.mask;
     p.err = ctx->d_err;
@@ -850,17 +858,17 @@ int launch_t(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs
     p.G = static_cast<uint32_t>(s.H / s.KVH);
     p.P = static_cast<uint32_t>(s.P);
     p.mask_words = static_cast<uint32_t>(s.mask_words);
-    p.slot_rows = v.slot_rows;
+    p.slot_rows = w.slot_rows;
     p.box_rows = box_rows;
     p.boxes = kTreeTile / box_rows;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.q_f32 = a.q_dtype == MLC_F32;
     p.o_f32 = a.o_dtype == MLC_F32;
-    MLCB_CUDA(ctx, launch_dependent(ctx, paged_tree_tcgen05_kernel<D, EXACT>, dim3(v.n_cta), kThreads, smem, mk, mv, p));
+    MLCB_CUDA(ctx, launch_dependent(ctx, paged_tree_tcgen05_kernel<D, EXACT>, dim3(w.n_cta), kThreads, smem, mk, mv, p));
     ++ctx->launches;
-    if (!v.n_slots) return MLC_OK;
-    if (a.o_dtype == MLC_F32) MLCB_CUDA(ctx, (merge_launch<D, float>(ctx, s, v, p.part_o, p.part_ml, a.o)));
-    else MLCB_CUDA(ctx, (merge_launch<D, __half>(ctx, s, v, p.part_o, p.part_ml, a.o)));
+    if (!w.n_slots) return MLC_OK;
+    if (a.o_dtype == MLC_F32) MLCB_CUDA(ctx, (merge_launch<D, float>(ctx, s, w, p.part_o, p.part_ml, a.o)));
+    else MLCB_CUDA(ctx, (merge_launch<D, __half>(ctx, s, w, p.part_o, p.part_ml, a.o)));
     ++ctx->launches;
     return MLC_OK;
 }

@@ -197,6 +197,22 @@ def test_plan_and_update(ex, dtype):
     plan.destroy()
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_one_plan_serves_both_types(ex, D):
+    """fp16 and fp32 calls, mixed ones too, on one plan without a wait in between."""
+    case = TreeCase(23, [3000, 90, 5], [20, 9, 1], 8, 2, D)
+    plan = plan_for(ex, case)
+    devs = [OnDevice(case, *t) for t in ((F16, F16), (F32, F32), (F16, F32), (F32, F16), (F16, F16))]
+    ex.beginForwardPassCB()
+    for d in devs:
+        assert ex.encodePagedTreeAttentionPlanned(plan, d.q, d.k, d.v, d.o, 0.0, d.q_dtype, d.o_dtype), ex.last_error()
+    assert ex.flushForwardPassCB(), ex.last_error()
+    for d in devs:
+        check(case, d, d.result(case))
+    assert ex.lastAttentionKernel() == 4
+    plan.destroy()
+
+
 def test_two_captured_graphs_and_eager_calls_share_the_context(ex):
     a, b = TreeCase(30, [4000, 100], [9, 3], 8, 2, 64), TreeCase(31, [9000], [30], 8, 2, 64)
     da, db = OnDevice(a), OnDevice(b)

@@ -7,12 +7,12 @@
 //
 // What bounds it: every logit is read once, so the memory's read bandwidth for large calls; a launch and the two chained
 // steps for small ones. One pass over the logits does both jobs: a warp walks a segment of a row, 512 logits a step with
-// the next step's in flight, and keeps a running maximum, a running sum of exponentials and the n_select largest logits
+// the next two steps' in flight, and keeps a running maximum, a running sum of exponentials and the n_select largest logits
 // so far; the last CTA of a group to finish joins the segments. Inside a row the order by score is the order by logit, so a
 // segment needs no logarithm. The largest logits are kept as a list in shared memory with a threshold, the n_select-th
 // largest at the last clean-up: on real logits few pass it after the first step, and a step in which none does costs one
-// vote. Warps work on their own: 512 rows of 128000, a quarter of them finished, take 64 us (the read of all of them 40); with a CTA
-// per 8192 logits and its five barriers it was 180.
+// vote. Warps work on their own: 512 rows of 128000, a quarter of them finished, take 61 us (the read
+// of all of them 40); with a CTA per 8192 logits and its five barriers it was 180, with the next step in registers 64.
 // The comparison between beams needs the differences of nearly equal sums: a lane's sum over a step is taken in fp32,
 // what joins the segments and the scores in fp64.
 #include <cuda_fp16.h>
@@ -27,8 +27,9 @@ namespace mlcb {
 namespace {
 
 constexpr uint32_t kThreads = 256, kWarps = kThreads / 32;
-constexpr uint32_t kCtasPerSm = 3;     // four would leave 64 registers a thread: 76 us instead of 63 for 512 rows of 128000
+constexpr uint32_t kCtasPerSm = 3;     // four, with room for two steps a warp: 62 us instead of 61 for 512 rows of 128000
 constexpr uint32_t kStep = 512;        // logits a warp takes at a time: four float4 a lane
+constexpr uint32_t kRing = 3;          // steps a warp has room for: two are under way while it works on one
 constexpr uint32_t kParts = 64;        // maxima a threshold is taken from
 constexpr uint32_t kMaxSelect = 64;    // = kParts: a threshold needs that many
 constexpr uint32_t kMaxBeams = 64;
@@ -120,11 +121,12 @@ __device__ __forceinline__ bool better(const Candidate& a, const Candidate& b) {
 }
 
 struct Shared {
-    uint32_t listed[kWarps];
     union {
-        uint64_t list[kWarps][kListCap];
+        float4 ring[kWarps][kRing][kStep / 4];   // logits on their way in
         Candidate found[kFoundCap];
     };
+    uint64_t list[kWarps][kListCap];
+    uint32_t listed[kWarps];
     float tops[kThreads];
     double lse[kMaxBeams];
     float part[kWarps][kParts];
@@ -283,12 +285,14 @@ __device__ __noinline__ uint32_t shorten(uint64_t* list, uint32_t n, uint32_t ke
     return shorten_to<kListCap / 32>(list, n, keep, lane);
 }
 
-// Sum of the exponentials of 16 logits on top of s, relative to the running maximum m; `quarter` receives the largest of every
-// four of them.
-__device__ __forceinline__ float add_step(const float (&x)[16], float& m, float& s, float (&quarter)[4]) {
+// The largest of every four of 16 logits, and of all of them; NaN is passed over.
+__device__ __forceinline__ float four_maxima(const float (&x)[16], float (&quarter)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) quarter[j] = fmaxf(max3(x[4 * j], x[4 * j + 1], x[4 * j + 2]), x[4 * j + 3]);   // passes over NaN
-    const float top = fmaxf(max3(quarter[0], quarter[1], quarter[2]), quarter[3]);
+    for (int j = 0; j < 4; ++j) quarter[j] = fmaxf(max3(x[4 * j], x[4 * j + 1], x[4 * j + 2]), x[4 * j + 3]);
+    return fmaxf(max3(quarter[0], quarter[1], quarter[2]), quarter[3]);
+}
+// Sum of the exponentials of 16 logits, the largest of which is `top`, on top of s, relative to the running maximum m.
+__device__ __forceinline__ void add_step(const float (&x)[16], float top, float& m, float& s) {
     const float both = fmaxf(m, top), ref = both == -INFINITY ? 0.f : both;
     const float2 minus = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
     float2 t[2] = {};
@@ -300,11 +304,11 @@ __device__ __forceinline__ float add_step(const float (&x)[16], float& m, float&
     t[0] = add2(t[0], t[1]);
     s = s * exp_diff(m, ref) + (t[0].x + t[0].y);
     m = both;
-    return top;
 }
 
 // One segment of a row, by one warp.
-__device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uint32_t* listed, float* part, uint32_t row, uint32_t seg, uint32_t lane) {
+__device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kStep / 4], uint64_t* list, uint32_t* listed, float* part,
+                                        uint32_t row, uint32_t seg, uint32_t lane) {
     const uint32_t block = seg / p.per_block, begin = (seg - block * p.per_block) * p.segment_len;
     const uint32_t block_rows = min(p.group_rows, p.vocab - block * p.group_rows);
     const int len = begin < block_rows ? static_cast<int>(min(p.segment_len, block_rows - begin)) : 0;   // the last block may be short
@@ -323,6 +327,19 @@ __device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uin
             x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
         }
     };
+    // A lane copies to shared memory what it will read itself: no registers wait for the logits, and nothing has to be synchronised
+    // but its own copies.
+    auto fetch = [&](int step) {
+        if (step < steps) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4* src = body + min(step * static_cast<int>(kStep / 4) + static_cast<int>(lane) + 32 * j, vecs - 1);
+                const uint32_t dst = static_cast<uint32_t>(__cvta_generic_to_shared(&ring[step % kRing][lane + 32 * j]));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     auto drop_behind = [&](int step, float (&x)[16]) {
         if ((step + 1) * static_cast<int>(kStep / 4) <= vecs) return;
 #pragma unroll
@@ -339,8 +356,8 @@ __device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uin
         threshold = fmaxf(threshold, key_value(lowest));
         __syncwarp();
     };
-    float next[16];
-    if (steps) load(0, next);
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(kRing) - 1; ++i) fetch(i);
     const int edge_at = static_cast<int>(lane) < head ? static_cast<int>(lane) : 4 * vecs + static_cast<int>(lane);
     const float edge = static_cast<int>(lane) < edges ? x0[edge_at] : -INFINITY;
     if (edges) {
@@ -356,22 +373,20 @@ __device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uin
 #pragma unroll 1
     for (int step = 0; step < steps; ++step) {
         float x[16];
+        asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = next[i];
-        if (step + 1 < steps) load(step + 1, next);
+        for (int j = 0; j < 4; ++j) {
+            const float4 v = ring[step % kRing][lane + 32 * j];
+            x[4 * j] = v.x; x[4 * j + 1] = v.y; x[4 * j + 2] = v.z; x[4 * j + 3] = v.w;
+        }
+        fetch(step + static_cast<int>(kRing) - 1);   // where the step before this one lay
         drop_behind(step, x);
         float quarter[4];
-        const float top = add_step(x, m, s, quarter);
-        if (step == 0) {
-            // The n_select-th largest of 64 maxima over parts of the step has that many logits at or above it.
-            float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                a = max3(a, x[i], x[i + 1]);
-                b = max3(b, x[8 + i], x[9 + i]);
-            }
-            part[lane] = a;
-            part[lane + 32] = b;
+        const float top = four_maxima(x, quarter);
+        add_step(x, top, m, s);
+        if (step == 0) {   // 64 disjoint parts: at least n_select logits reach the n_select-th largest of their maxima
+            part[lane] = fmaxf(quarter[0], quarter[1]);
+            part[lane + 32] = fmaxf(quarter[2], quarter[3]);
             __syncwarp();
             threshold = fmaxf(kLowest, kth_of_64(part, p.n_select, lane));
         }
@@ -422,7 +437,7 @@ __device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uin
             for (int i = 0; i < 16; ++i)
                 if (!(x[i] == x[i])) x[i] = -INFINITY;
             float quarter[4];
-            add_step(x, m, s, quarter);
+            add_step(x, four_maxima(x, quarter), m, s);
         }
     }
     float top = m;
@@ -438,15 +453,17 @@ __device__ __forceinline__ void segment(const BeamParams& p, uint64_t* list, uin
 }
 
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) beam_select_kernel(const __grid_constant__ BeamParams p) {
-    __shared__ Shared sh;
+    extern __shared__ __align__(16) uint8_t smem[];
+    Shared& sh = *reinterpret_cast<Shared*>(smem);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t group = blockIdx.x / p.ctas_per_group;
-    const uint32_t unit = (blockIdx.x - group * p.ctas_per_group) * kWarps + warp;   // (beam, segment) of the group
+    // (beam, segment) of the group; a CTA's warps are far apart, so that every CTA has its share of a finished beam's idle ones
+    const uint32_t unit = warp * p.ctas_per_group + (blockIdx.x - group * p.ctas_per_group);
     if (unit < p.beams * p.segments) {
         const uint32_t row = group * p.beams + unit / p.segments;
-        if (!p.finished || !p.finished[row]) segment(p, sh.list[warp], &sh.listed[warp], sh.part[warp], row, unit % p.segments, lane);
+        if (!p.finished || !p.finished[row]) segment(p, sh.ring[warp], sh.list[warp], &sh.listed[warp], sh.part[warp], row, unit % p.segments, lane);
     }
     // the last CTA of the group joins: thread 0 publishes what the CTA wrote, and sees what the others published
     __syncthreads();
@@ -476,8 +493,8 @@ int beam_select(mlc_ctx* ctx, const void* logits, const void* cum, const void* f
         return ctx->fail(MLC_ERR_INVALID_ARG, "buffers must be aligned to their elements");
     if (group_rows == 0 || group_rows > vocab) group_rows = vocab;
     const size_t rows = groups * beams, blocks = (vocab + group_rows - 1) / group_rows;
-    // Segments: enough to give every SM its warps once (twice as many take 68 us instead of 63), but no more lists per group than one CTA joins in a few
-    // microseconds, and at least a step each.
+    // Segments: enough to give every SM its warps once (twice as many take 68 us instead of 61), but no more lists per
+    // group than one CTA joins in a few microseconds, and at least a step each.
     const size_t wanted = std::min<size_t>(static_cast<size_t>(ctx->sm_count) * kCtasPerSm * kWarps / rows, kMaxLists / beams);
     size_t per_block = std::min<size_t>(std::max<size_t>(wanted / blocks, 1), (group_rows + kStep - 1) / kStep);
     const size_t segment_len = ((group_rows + per_block - 1) / per_block + 3) / 4 * 4;
@@ -512,7 +529,12 @@ int beam_select(mlc_ctx* ctx, const void* logits, const void* cum, const void* f
     p.ctas_per_group = static_cast<uint32_t>(ctas_per_group);
     p.n_select = static_cast<uint32_t>(n_select);
     p.pad = pad_token;
-    MLCB_CUDA(ctx, launch_dependent(ctx, beam_select_kernel, dim3(static_cast<unsigned>(groups * ctas_per_group)), kThreads, 0, p));
+    if (!ctx->beam_smem_set) {
+        MLCB_CUDA(ctx, cudaFuncSetAttribute(beam_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(Shared))));
+        ctx->beam_smem_set = true;
+    }
+    static_assert((sizeof(Shared) + 1024) * kCtasPerSm <= 228 * 1024, "CTAs per SM");
+    MLCB_CUDA(ctx, launch_dependent(ctx, beam_select_kernel, dim3(static_cast<unsigned>(groups * ctas_per_group)), kThreads, sizeof(Shared), p));
     ++ctx->launches;
     return MLC_OK;
 }

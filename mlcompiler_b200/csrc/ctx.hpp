@@ -91,6 +91,7 @@ struct mlc_ctx {
     size_t n_counters = 0;
     size_t decode_smem_set[16] = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};  // dynamic-smem opt-in already applied, per kernel variant
     bool tree_smem_set[4] = {false, false, false, false};   // same, for the variants of the tree attention kernel
+    bool beam_smem_set = false;                // same, for beam selection
     bool prefill_smem_set = false;             // same, for the chunked-prefill kernel
     // copy streams and events of the host-buffer decode pass (created on first use)
     cudaStream_t h2d_stream = nullptr, d2h_stream = nullptr;

@@ -62,7 +62,8 @@ struct Config {
 template <uint32_t STAGES>
 struct Bars {
     uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES], s_full[2], p_full[2], pv_done;
-    uint32_t tmem_slot, not_finite;
+    uint32_t tmem_slot;
+    uint32_t not_finite[2];   // pieces in turn: a warp may be in the next one before another has read the last one's
 };
 
 struct TreeParams {
@@ -321,7 +322,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             tc::mbar_init(smem_u32(&bars.p_full[b]), 128);   // two, like the S buffers: softmax may be a tile ahead of the MMA warp
         }
         tc::mbar_init(smem_u32(&bars.pv_done), 1);
-        bars.not_finite = 0;
+        bars.not_finite[0] = bars.not_finite[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 4) tc::tmem_alloc(smem_u32(&bars.tmem_slot), C::tmem_cols);
@@ -643,7 +644,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                         }
                         if (any) {
                             st_shared16(addr, x);
-                            *reinterpret_cast<volatile uint32_t*>(&bars.not_finite) = pi + 1;
+                            *reinterpret_cast<volatile uint32_t*>(&bars.not_finite[pi & 1u]) = pi + 1;
                         }
                     }
                     tc::fence_proxy_async_smem();
@@ -675,7 +676,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 const float inv = whole ? (l_sum == 0.f ? 0.f : 1.0f / l_sum) : 1.0f;
                 const size_t out = (static_cast<size_t>(done.token0 + r / prm.G) * prm.H + done.kv_head * prm.G + r % prm.G) * D;
                 const size_t part = static_cast<size_t>(done.slot) * prm.slot_rows + row;
-                const bool repair = *reinterpret_cast<volatile uint32_t*>(&bars.not_finite) == pi + 1;
+                const bool repair = *reinterpret_cast<volatile uint32_t*>(&bars.not_finite[pi & 1u]) == pi + 1;
                 if (!whole && mine) prm.part_ml[part] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * scale, l_sum);
                 // drafted tokens of this piece that the row sees: what is not finite in V belongs in its output
                 auto put_back = [&](int c0, uint32_t (&o)[32]) {

@@ -460,8 +460,8 @@ int mlc_encode_argmax_rows(mlc_ctx* ctx, const void* logits, size_t batch, size_
  * (uint32 t), each [groups, n_select], best first; equal scores: the lower p, then the lower t. finished (device
  * uint8 [groups, beams], may be NULL): a beam with a nonzero entry has one candidate, (p, pad_token) with its score
  * as it is, and its logits are not read. Candidates whose score is -inf or not a number (a logit of -inf or NaN, a row
- * with a +inf) are never selected; places that stay empty get -inf and 0xFFFFFFFF. beams and n_select <= 64
- * (MLC_ERR_UNSUPPORTED). Capturable once the call has run outside a capture. */
+ * with a +inf) are never selected; places that stay empty get -inf and 0xFFFFFFFF. Outputs must not overlap
+ * the inputs or each other (MLC_ERR_INVALID_ARG). beams and n_select <= 64 (MLC_ERR_UNSUPPORTED). Capturable once the call has run outside a capture. */
 int mlc_encode_beam_select(mlc_ctx* ctx, const void* logits, const void* cum_scores, const void* finished, size_t groups,
                            size_t beams, size_t vocab, size_t group_rows, size_t n_select, uint32_t pad_token,
                            void* out_scores, void* out_parents, void* out_tokens);
@@ -534,7 +534,7 @@ int mlc_encode_paged_prefill_attention(mlc_ctx* ctx, const void* q, const void* 
  * lies in rows that a token does not see - other branches, slots behind the last token - has no
  * effect on it, infinities and NaN included.
  *   q, o          device [sum_r draft_lens[r], num_heads, head_dim], request after request, fp16 or
- *                 fp32 per q_dtype / o_dtype
+ *                 fp32 per q_dtype / o_dtype; they must not overlap (MLC_ERR_INVALID_ARG)
  *   tree_mask     host u32 [sum_r draft_lens[r], mask_words]: bit j of row i (word j / 32, bit
  *                 j % 32) set = drafted token i sees drafted token j of its request. A tree sets a
  *                 token's own bit and its ancestors'. Bits at or above draft_lens[r] are ignored;

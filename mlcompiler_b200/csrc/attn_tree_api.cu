@@ -160,6 +160,9 @@ int check_call(mlc_ctx* ctx, const TreeArgs& a) {
 
 int launch(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, TreeArgs a) {
     if (s.tokens == 0) return MLC_OK;
+    const size_t elems = s.tokens * s.H * s.D;
+    if (overlap(a.q, elems * (a.q_dtype == MLC_F32 ? 4 : 2), a.o, elems * (a.o_dtype == MLC_F32 ? 4 : 2)))
+        return ctx->fail(MLC_ERR_INVALID_ARG, "o overlaps q");
     if (!(a.scale > 0.f)) a.scale = 1.0f / std::sqrt(static_cast<float>(s.D));
     if (v.work[0].n_cta && !ctx->force_general && tree_tcgen05_buffers(a)) {
         ctx->last_attention_kernel = 4;

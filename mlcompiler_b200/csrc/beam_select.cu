@@ -504,6 +504,16 @@ int beam_select(mlc_ctx* ctx, const void* logits, const void* cum, const void* f
     if (rows * segments >= (size_t(1) << 31) || groups * ctas_per_group >= (size_t(1) << 31) ||
         beams * segments * n_select >= (size_t(1) << 31))
         return ctx->fail(MLC_ERR_UNSUPPORTED, "too many rows");
+    // a group may still read its scores when another one has written its results
+    struct { const void* at; size_t bytes; } in[] = {{logits, rows * vocab * 4}, {cum, rows * 4}, {finished, finished ? rows : 0}};
+    const void* out[] = {out_scores, out_parents, out_tokens};
+    const size_t out_bytes = groups * n_select * 4;
+    for (size_t i = 0; i < 3; ++i) {
+        for (const auto& x : in)
+            if (overlap(out[i], out_bytes, x.at, x.bytes)) return ctx->fail(MLC_ERR_INVALID_ARG, "an output overlaps an input");
+        for (size_t j = 0; j < i; ++j)
+            if (overlap(out[i], out_bytes, out[j], out_bytes)) return ctx->fail(MLC_ERR_INVALID_ARG, "two outputs overlap");
+    }
     DeviceGuard guard(ctx->device);
     const size_t key_bytes = rows * segments * n_select * 8, sum_bytes = rows * segments * sizeof(float2);
     int st = ensure_op_scratch(ctx, ctx->beam_scratch, key_bytes + sum_bytes, "beam selection scratch");

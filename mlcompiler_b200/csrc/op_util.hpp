@@ -31,6 +31,10 @@ int ensure_op_scratch(mlc_ctx* ctx, OpScratch& s, size_t bytes, const char* what
 // from them before everything in front of it has finished.
 void note_pool_writes(mlc_ctx* ctx, void* const* pools, size_t n_pools);
 
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
 inline bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 // Launch as a programmatic dependent of the kernel in front: the kernel waits (griddepcontrol.wait) before it touches

@@ -240,3 +240,19 @@ def test_refusals(ex):
     assert call(done=done, pad=10) == 1 and call(done=done, pad=9) == 0 and call(pad=10) == 0
     assert call(s=s.data_ptr() + 1) == 1
     assert ex.flushForwardPassCB()
+
+
+def test_overlapping_buffers_are_refused(ex):
+    import torch
+    x, c = torch.zeros(2, 10, device="cuda"), torch.zeros(1, 2, device="cuda")
+    done = torch.zeros(8, dtype=torch.uint8, device="cuda")
+    s, p, t = (torch.zeros(2, dtype=d, device="cuda") for d in (torch.float32, torch.int32, torch.int32))
+
+    def call(x=x, c=c, done=None, s=s, p=p, t=t):
+        return 0 if ex.encodeBeamSelect(x, c, done, 1, 2, 10, 0, 2, 0, s, p, t) else ex.last_status
+
+    ex.beginForwardPassCB()
+    assert call(s=c) == 1 and call(t=x) == 1 and call(p=x.data_ptr() + 76) == 1 and call(done=done, p=done) == 1
+    assert call(p=t) == 1 and call(s=t.data_ptr() + 4) == 1
+    assert call() == 0 and call(done=done) == 0
+    assert ex.flushForwardPassCB()

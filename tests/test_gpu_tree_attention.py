@@ -326,3 +326,32 @@ def test_tree_mask_from_parents():
     assert capi.Executor.treeMask([list(range(-1, 39))]).shape == (40, 2)
     with pytest.raises(ValueError):
         capi.Executor.treeMask([[0]])
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_infinite_values_in_every_run_of_a_cta(ex, dtype):
+    """More (request, KV head) runs than CTAs: each CTA works through several, every one with an infinite value of its own."""
+    rng = np.random.default_rng(70)
+    prefix = rng.integers(0, 130, 700)
+    case = TreeCase(71, prefix.tolist(), [4] * 700, 2, 2, 64, mask="chain")
+    for r in range(case.N):
+        page, slot = case.where(r, int(prefix[r]) + 2)
+        case.v[page, slot, r % 2, r % 64] = np.inf
+    _, got = run(ex, case, dtype, dtype)
+    want = np.zeros(got.shape, bool)
+    for r in range(case.N):
+        want[4 * r + 2: 4 * r + 4, r % 2, r % 64] = True
+    assert (np.isposinf(got) == want).all() and np.isfinite(got[~want]).all()
+
+
+def test_output_over_the_queries_is_refused(ex):
+    case = TreeCase(72, [40], [3], 4, 2, 64)
+    dev = OnDevice(case)
+    plan = plan_for(ex, case)
+    ex.beginForwardPassCB()
+    assert not ex.encodePagedTreeAttentionPlanned(plan, dev.q, dev.k, dev.v, dev.q) and ex.last_status == 1
+    assert not ex.encodePagedTreeAttentionPlanned(plan, dev.q, dev.k, dev.v, dev.q.data_ptr() + 16) and ex.last_status == 1
+    assert ex.encodePagedTreeAttentionPlanned(plan, dev.q, dev.k, dev.v, dev.o)
+    assert ex.flushForwardPassCB()
+    check(case, dev, dev.result(case))
+    plan.destroy()

@@ -15,9 +15,9 @@ namespace mlcb {
 
 namespace {
 
-// Tiles a piece's fixed work (queries in, output or partial out) counts for: 32 requests of 1 to 4095 tokens take 36.9 us
-// with 2, 35.8 with 4.
-constexpr uint32_t kPieceCost = 4;
+// Tiles a piece's fixed work (queries in, output or partial out) counts for: 32 requests of 1 to 4095 tokens take 32.7 us
+// with 3, 32.0 with 4, 31.7 with 5.
+constexpr uint32_t kPieceCost = 5;
 // No cut leaves less than this. One request of 1000 tokens, 8 drafted: 8.8 us with 2, 9.5 with 4, 11.6 with 8.
 constexpr uint32_t kMinPiece = 2;
 // Where every run has a CTA of its own and none is longer than this, nothing is cut: the second kernel costs more than

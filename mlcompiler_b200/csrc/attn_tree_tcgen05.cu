@@ -733,63 +733,69 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     if (warp == 4) tc::tmem_dealloc(tmem, C::tmem_cols);
 }
 
-// O of the rows whose run was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. WARPS warps per row
-// take the parts round-robin, eight in flight at a time. The tables are read before the wait for the kernel in front.
-template <int D, int WARPS, typename OT>
-__global__ void __launch_bounds__(128) tree_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml,
-                                                         const TreeSplit* __restrict__ splits, const uint32_t* __restrict__ row_split,
-                                                         OT* __restrict__ o, uint32_t rows, uint32_t slot_rows, uint32_t H, uint32_t G) {
-    constexpr int kLanes = D / 4;               // lanes a part's row takes, four columns each
-    constexpr int kAtOnce = 32 / kLanes;        // parts a warp reads with one instruction
-    constexpr int kStride = WARPS * kAtOnce;
-    __shared__ float4 s_o[WARPS > 1 ? WARPS : 1][kLanes];
-    __shared__ float s_l[4];
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t row = blockIdx.x * (4 / WARPS) + warp / WARPS, sub = warp % WARPS;
-    if (row >= rows) return;   // with WARPS > 1 a CTA has one row: all or none leave
+// O of the rows whose run was cut: sum_k o_k 2^(m_k - m) / sum_k l_k 2^(m_k - m), parts in fixed order. A row has SHARES groups of
+// D / 4 threads, four columns a thread; a group takes every SHARES-th part, four in flight. The tables are read before the
+// wait for the kernel in front.
+constexpr uint32_t merge_rows_per_cta(int D, int shares) { return D / 4 * shares < 128 ? 512 / (D * shares) : 1; }
+
+template <int D, int SHARES, typename OT>
+__global__ void __launch_bounds__(D / 4 * SHARES * merge_rows_per_cta(D, SHARES))
+tree_merge_kernel(const float* __restrict__ part_o, const float2* __restrict__ part_ml, const TreeSplit* __restrict__ splits,
+                  const uint32_t* __restrict__ row_split, OT* __restrict__ o, uint32_t rows, uint32_t slot_rows, uint32_t H, uint32_t G) {
+    constexpr uint32_t kLanes = D / 4, kFlight = 4, kRows = merge_rows_per_cta(D, SHARES);
+    __shared__ float4 s_o[kRows][SHARES][kLanes];
+    __shared__ float2 s_ml[kRows][SHARES];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t column = threadIdx.x % kLanes, share = threadIdx.x / kLanes % SHARES, in_cta = threadIdx.x / (kLanes * SHARES);
+    const uint32_t row = min(blockIdx.x * kRows + in_cta, rows - 1);   // (the last CTA may work on the last row several times)
     const TreeSplit sp = splits[row_split[row]];
     const uint32_t r = row - sp.first_row;
     auto index = [&](uint32_t k) { return static_cast<size_t>(sp.first_slot + k * sp.slot_step) * slot_rows + r; };
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    float top = -INFINITY;
-    for (uint32_t k = lane; k < sp.n_parts; k += 32) top = fmaxf(top, __ldcg(&part_ml[index(k)]).x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float top = -INFINITY, l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
-#pragma unroll 8
-    for (uint32_t k = sub * kAtOnce + lane / kLanes; k < sp.n_parts; k += kStride) {
-        const float2 ml = __ldcg(&part_ml[index(k)]);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(part_o + index(k) * D) + lane % kLanes);
-        // a part that saw nothing has m = -inf, l = 0 and o = 0
+    auto add = [&](float2 ml, float4 v) {   // a part that saw nothing has m = -inf, l = 0 and o = 0
         const float w = ml.x == -INFINITY ? 1.0f : ex2(ml.x - top);
         l += ml.y * w;
         acc.x += v.x * w; acc.y += v.y * w; acc.z += v.z * w; acc.w += v.w * w;
+    };
+    for (uint32_t k0 = share; k0 < sp.n_parts; k0 += SHARES * kFlight) {
+        float2 ml[kFlight];
+        float4 v[kFlight];
+#pragma unroll
+        for (uint32_t i = 0; i < kFlight; ++i) {
+            const uint32_t k = k0 + i * SHARES;
+            ml[i] = make_float2(-INFINITY, 0.f);
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < sp.n_parts) {
+                ml[i] = __ldcg(&part_ml[index(k)]);
+                v[i] = __ldcg(reinterpret_cast<const float4*>(part_o + index(k) * D) + column);
+            }
+        }
+        float both = top;
+#pragma unroll
+        for (uint32_t i = 0; i < kFlight; ++i) both = fmaxf(both, ml[i].x);
+        const float w = top == -INFINITY ? 0.f : ex2(top - both);
+        top = both;
+        l *= w;
+        acc.x *= w; acc.y *= w; acc.z *= w; acc.w *= w;
+#pragma unroll
+        for (uint32_t i = 0; i < kFlight; ++i) add(ml[i], v[i]);
     }
-    if constexpr (kAtOnce == 2) {
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        acc.x += __shfl_xor_sync(0xffffffffu, acc.x, 16);
-        acc.y += __shfl_xor_sync(0xffffffffu, acc.y, 16);
-        acc.z += __shfl_xor_sync(0xffffffffu, acc.z, 16);
-        acc.w += __shfl_xor_sync(0xffffffffu, acc.w, 16);
-    }
-    if constexpr (WARPS > 1) {
-        if (lane == 0) s_l[warp] = l;
-        if (lane < kLanes) s_o[sub][lane] = acc;
+    if constexpr (SHARES > 1) {
+        if (column == 0) s_ml[in_cta][share] = make_float2(top, l);
+        s_o[in_cta][share][column] = acc;
         __syncthreads();
-        if (sub) return;
+        if (share) return;
+        for (int i = 1; i < SHARES; ++i) top = fmaxf(top, s_ml[in_cta][i].x);
         l = 0.f;
         acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < WARPS; ++w) {
-            const float4 v = s_o[w][lane % kLanes];
-            l += s_l[w];
-            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
-        }
+#pragma unroll
+        for (int i = 0; i < SHARES; ++i) add(s_ml[in_cta][i], s_o[in_cta][i][column]);
     }
-    if (lane >= kLanes) return;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const uint32_t rr = sp.row_begin + r;
-    OT* dst = o + (static_cast<size_t>(sp.token0 + rr / G) * H + sp.kv_head * G + rr % G) * D + lane * 4;
+    OT* dst = o + (static_cast<size_t>(sp.token0 + rr / G) * H + sp.kv_head * G + rr % G) * D + column * 4;
     if constexpr (sizeof(OT) == 4) *reinterpret_cast<float4*>(dst) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     else *reinterpret_cast<uint2*>(dst) = make_uint2(pack(acc.x * inv, acc.y * inv), pack(acc.z * inv, acc.w * inv));
 }
@@ -817,12 +823,20 @@ int pool_map(mlc_ctx* ctx, CUtensorMap* out, const void* pool, const TreeShape& 
 
 template <int D, typename OT>
 cudaError_t merge_launch(mlc_ctx* ctx, const TreeShape& s, const TreeWorkView& v, const float* part_o, const float2* part_ml, void* o) {
-    // many parts a row: four warps share it
-    const bool wide = v.max_parts > 8;
-    auto kernel = wide ? tree_merge_kernel<D, 4, OT> : tree_merge_kernel<D, 1, OT>;
-    const dim3 grid(wide ? v.merge_rows : (v.merge_rows + 3) / 4);
-    return launch_dependent(ctx, kernel, grid, 128, 0, part_o, part_ml, v.splits, v.row_split, static_cast<OT*>(o), v.merge_rows,
-                            v.slot_rows, static_cast<uint32_t>(s.H), static_cast<uint32_t>(s.H / s.KVH));
+    auto go = [&](auto n_shares) {
+        constexpr int SHARES = decltype(n_shares)::value;
+        constexpr uint32_t kRows = merge_rows_per_cta(D, SHARES);
+        return launch_dependent(ctx, tree_merge_kernel<D, SHARES, OT>, dim3((v.merge_rows + kRows - 1) / kRows), D / 4 * SHARES * kRows, 0,
+                                part_o, part_ml, v.splits, v.row_split, static_cast<OT*>(o), v.merge_rows, v.slot_rows,
+                                static_cast<uint32_t>(s.H), static_cast<uint32_t>(s.H / s.KVH));
+    };
+    // More threads a row where there are parts for them and room: beyond the threads that are resident at once, the waiting
+    // of a second wave costs more.
+    const uint64_t room = static_cast<uint64_t>(ctx->sm_count) * 1280 / (static_cast<uint64_t>(v.merge_rows) * (D / 4));
+    constexpr int kMost = D == 64 ? 16 : 8;
+    if (v.max_parts > 16 && room >= kMost) return go(Blocks<kMost>());
+    if (v.max_parts > 4 && room >= 4) return go(Blocks<4>());
+    return go(Blocks<1>());
 }
 
 template <int D, bool EXACT>

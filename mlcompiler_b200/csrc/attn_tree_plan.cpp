@@ -18,11 +18,11 @@ namespace {
 // Tiles a piece's fixed work (queries in, output or partial out) counts for: 32 requests of 1 to 4095 tokens take 32.7 us
 // with 3, 32.0 with 4, 31.7 with 5.
 constexpr uint32_t kPieceCost = 5;
-// No cut leaves less than this. One request of 1000 tokens, 8 drafted: 8.8 us with 2, 9.5 with 4, 11.6 with 8.
+// No cut leaves less than this. One request of 1000 tokens, 8 drafted: 7.7 us with 2, 8.6 with 4.
 constexpr uint32_t kMinPiece = 2;
 // Where every run has a CTA of its own and none is longer than this, nothing is cut: the second kernel costs more than
-// the tiles it saves. 16 requests of 500 tokens (8 tiles): 9.0 us whole, 11.6 cut; one of 1000 (16 tiles): 12.9 whole, 8.8 cut.
-constexpr uint32_t kWholeTiles = 9;
+// the tiles it saves. 16 requests of 300 tokens (5 tiles): 8.0 us whole, 9.4 cut; of 500 (8 tiles): 10.5 whole, 9.1 cut.
+constexpr uint32_t kWholeTiles = 6;
 constexpr uint32_t kLanes = 8;
 
 }  // namespace

@@ -662,9 +662,9 @@ void mlc_exchange_destroy(mlc_ctx* ctx, mlc_exchange* ex);
 /* ---- CUDA-graph bracketing of a pass --------------------------------------------------
  * Records the planned encode_* calls issued between begin and end into a CUDA graph
  * that replays them with one launch (the reference pays one command-buffer commit
- * per pass, metal_runtime.mm:6030-6033). Only the *_planned entry points and
- * mlc_encode_lse_combine may be called while capturing; run the same sequence once
- * outside a capture first so that workspaces exist. */
+ * per pass, metal_runtime.mm:6030-6033). Only the *_planned entry points,
+ * mlc_encode_lse_combine and mlc_encode_beam_select may be called while capturing; run the
+ * same sequence once outside a capture first so that workspaces exist. */
 typedef struct mlc_graph mlc_graph;
 int mlc_graph_begin_capture(mlc_ctx* ctx);
 int mlc_graph_end_capture(mlc_ctx* ctx, mlc_graph** out);

@@ -333,8 +333,17 @@ int mlc_tree_plan_update(mlc_ctx* ctx, mlc_tree_plan* plan, const uint32_t* page
 void mlc_tree_plan_destroy(mlc_ctx* ctx, mlc_tree_plan* plan) {
     if (!ctx || !plan) return;
     DeviceGuard guard(ctx->device);
-    cudaStreamSynchronize(ctx->stream);
-    release_buffers(*plan);
+    if (ctx->capturing) {
+        // waiting or freeing here would spoil the capture: the buffers go with the context
+        no_throw(ctx, [&] {
+            if (plan->dev) ctx->tree_scratch.retired.push_back(plan->dev);
+            if (plan->host) ctx->tree_scratch.retired_host.push_back(plan->host);
+            return MLC_OK;
+        });
+    } else {
+        cudaStreamSynchronize(ctx->stream);
+        release_buffers(*plan);
+    }
     if (plan->uploaded) cudaEventDestroy(plan->uploaded);
     delete plan;
 }

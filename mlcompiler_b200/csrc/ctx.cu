@@ -123,6 +123,7 @@ int ensure_op_scratch(mlc_ctx* ctx, OpScratch& s, size_t bytes, const char* what
 
 static void free_op_scratch(OpScratch& s) {
     for (void* p : s.retired) cudaFree(p);
+    for (void* p : s.retired_host) cudaFreeHost(p);
     if (s.dev) cudaFree(s.dev);
     s = OpScratch();
 }

@@ -51,7 +51,7 @@ struct ExchangeView {
 struct OpScratch {
     void* dev = nullptr;
     size_t bytes = 0;
-    std::vector<void*> retired;
+    std::vector<void*> retired, retired_host;   // device and page-locked memory that goes with the context
 };
 
 struct AttnPlanCache;  // attn_api.cu

@@ -256,3 +256,29 @@ def test_overlapping_buffers_are_refused(ex):
     assert call(p=t) == 1 and call(s=t.data_ptr() + 4) == 1
     assert call() == 0 and call(done=done) == 0
     assert ex.flushForwardPassCB()
+
+
+def test_logits_beyond_four_gigabytes(ex):
+    """All logits 0 but one of 5 per row, so a row's best score is its cumulated one plus 5 - log(V - 1 + e^5)."""
+    import torch
+    G, B, V, n = 64, 64, 270001, 5
+    x = torch.zeros((G * B, V), device="cuda")
+    assert x.numel() * 4 > 1 << 32
+    rng = np.random.default_rng(40)
+    token = rng.integers(0, V, G * B)
+    x[torch.arange(G * B, device="cuda"), torch.from_numpy(token).cuda()] = 5.0
+    cum = (rng.permutation(G * B) * 2.0**-9).astype(np.float32).reshape(G, B)   # distinct, and below 8: the next token of a beam is 5 behind
+    dev = [torch.from_numpy(cum).cuda(), torch.zeros((G, n), device="cuda")] + [torch.zeros((G, n), dtype=torch.int32, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    ex.beginForwardPassCB()
+    assert ex.encodeBeamSelect(x, dev[0], None, G, B, V, 0, n, 0, *dev[1:]), ex.last_error()
+    assert ex.flushForwardPassCB(), ex.last_error()
+    best = np.argsort(-cum, axis=1, kind="stable")[:, :n]
+    assert (dev[2].cpu().numpy() == best).all()
+    assert (dev[3].cpu().numpy() == token.reshape(G, B)[np.arange(G)[:, None], best]).all()
+    want = np.take_along_axis(cum.astype(np.float64), best, 1) + 5.0 - np.log(V - 1 + np.exp(5.0))
+    # The sum's relative error is the logarithm's absolute one. A lane adds up 528 steps in fp32 (2^-24 of the sum each at most, and
+    # as much for the 4 additions inside a step); an exponential is off by 2^-22 and by its argument's rounding, 5 * 2^-24; so are the
+    # two factors that bring lane and row to one maximum. The score is rounded once.
+    tol = (528 + 4 + 3 * 9) * 2.0**-24 + 2.0**-24 * np.abs(want).max()
+    assert np.abs(dev[1].cpu().numpy() - want).max() <= tol

@@ -159,3 +159,26 @@ def test_compact_refusals(ex):
     assert (now(keep, 0, host.shape[1:]) == host).all()
     assert call(kept=(0, 1, 0)) == 0                                     # nothing moves
     assert (now(keep, 0, host.shape[1:]) == host).all()
+
+
+def test_pages_and_rows_beyond_four_gigabytes(ex):
+    import torch
+    P, KVH, D = 64, 8, 128
+    capacity = (1 << 32) // (P * KVH * D * 2) + 8
+    pool = torch.empty((capacity, P, KVH, D), dtype=torch.int16, device="cuda")
+    pool[-8:] = torch.randint(-32768, 32767, (8, P, KVH, D), dtype=torch.int16, device="cuda")
+    pool[:2] = 7
+    before = pool[-8:].cpu().numpy()
+    torch.cuda.synchronize()
+    ptrs = capi.Executor.pointerArray([pool.data_ptr()])
+    assert ex.copyKVPages(ptrs, [capacity - 1, capacity - 2], [0, capacity - 8], P, KVH, D, 2, capacity), ex.last_error()
+    assert ex.compactKVRows(ptrs, [capacity - 4, capacity - 3], [0, 2], [60], [1, 5, 7], [0, 3], 1, P, KVH, D, 2, capacity), ex.last_error()
+    torch.cuda.synchronize()
+    want = before.copy()
+    want[0] = before[6]
+    rows = before[4:6].reshape(2 * P, KVH, D)
+    moved = rows.copy()
+    moved[60:63] = rows[[61, 65, 67]]
+    want[4:6] = moved.reshape(2, P, KVH, D)
+    assert (pool[-8:].cpu().numpy() == want).all()
+    assert (pool[0].cpu().numpy() == before[7]).all() and (pool[1] == 7).all()

@@ -355,3 +355,52 @@ def test_output_over_the_queries_is_refused(ex):
     assert ex.flushForwardPassCB()
     check(case, dev, dev.result(case))
     plan.destroy()
+
+
+def test_a_plan_goes_while_another_call_is_captured(ex):
+    case = TreeCase(73, [700], [9], 8, 2, 64)
+    dev = OnDevice(case)
+    plan, other = plan_for(ex, case), plan_for(ex, case)
+    ex.beginForwardPassCB()
+    assert ex.encodePagedTreeAttentionPlanned(plan, dev.q, dev.k, dev.v, dev.o), ex.last_error()
+    assert ex.beginCapture()
+    other.destroy()
+    assert ex.encodePagedTreeAttentionPlanned(plan, dev.q, dev.k, dev.v, dev.o), ex.last_error()
+    graph = ex.endCapture()
+    assert ex.flushForwardPassCB(), ex.last_error()
+    dev.o[: case.T].zero_()
+    import torch
+    torch.cuda.synchronize()
+    graph.launch()
+    check(case, dev, dev.result(case))
+    graph.destroy()
+    plan.destroy()
+
+
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_more_heads_in_a_group_than_a_row_tile_holds(ex, dtype):
+    case = TreeCase(74, [100, 3], [5, 2], 200, 1, 64)
+    check(case, *run(ex, case, dtype, dtype))
+    case = TreeCase(75, [30], [3], 260, 2, 128)
+    check(case, *run(ex, case, dtype, dtype))
+
+
+@pytest.mark.parametrize("D,KVH", [(64, 8), (80, 8)])
+def test_pages_beyond_four_gigabytes(ex, D, KVH):
+    """Pools of more than 2^32 bytes, the request's pages at their far end (the rest is left as it is)."""
+    import torch
+    case = TreeCase(76, [150], [5], 16, KVH, D)
+    bytes_per_page = 64 * KVH * D * 2
+    capacity = (1 << 32) // bytes_per_page + 1000
+    dev = OnDevice(case)
+    pools = []
+    for host in (case.k, case.v):
+        pool = torch.empty((capacity, 64, KVH, D), dtype=torch.float16, device="cuda")
+        pool[capacity - case.capacity:] = torch.from_numpy(host).cuda()
+        pools.append(pool)
+    torch.cuda.synchronize()
+    flat, off, prefix, draft, mask = case.tables()
+    assert ex.runPagedTreeAttention(dev.q, *pools, dev.o, flat + np.uint32(capacity - case.capacity), off, prefix, draft, mask, 1, 16, KVH, D,
+                                    64, 0.0, F16, F16, capacity), ex.last_error()
+    assert ex.lastAttentionKernel() == (4 if D == 64 else 1)
+    check(case, dev, dev.result(case))

@@ -593,7 +593,8 @@ int mlc_encode_copy_kv_pages(mlc_ctx* ctx, void* const* pools, size_t n_pools, c
  * positions start_positions[r] + i, as if every source were read before any destination is
  * written. A request's kept rows must rise strictly (MLC_ERR_INVALID_ARG) and lie inside its pages
  * (MLC_ERR_BOUNDS). Rows behind the last kept one keep their bytes. Two requests must not touch
- * the same page where rows move (MLC_ERR_INVALID_ARG: copy a shared page first). */
+ * the same page where rows move, nor may one request have it twice there (MLC_ERR_INVALID_ARG: copy
+ * a shared page first). */
 int mlc_run_compact_kv_rows(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* page_tables_flat,
                             size_t n_page_tables_flat, const uint32_t* page_table_offsets,
                             const uint32_t* start_positions, const uint32_t* kept_rows, const uint32_t* kept_offsets,

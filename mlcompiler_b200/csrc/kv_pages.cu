@@ -263,13 +263,14 @@ int compact_rows(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, co
                 return ctx->fail(MLC_ERR_BOUNDS, "kept row %u of request %zu lies behind its %u pages", list[i], r, pt_off[r + 1] - pt_off[r]);
             if (from == to) continue;
             const uint32_t src_page = table[from / P], dst_page = table[to / P];
-            for (const uint32_t id : {src_page, dst_page}) {
+            for (const uint64_t pos : {from, to}) {
+                const uint32_t at = static_cast<uint32_t>(pos / P), id = table[at];
                 if (cap && id >= cap)
                     return ctx->fail(MLC_ERR_BOUNDS, "page id %u of request %zu >= capacity %zu", id, r, cap);
-                // the requests run side by side: none may touch a page whose rows another one moves
-                const uint32_t owner = owners.claim(id, static_cast<uint32_t>(r));
-                if (owner != r)
-                    return ctx->fail(MLC_ERR_INVALID_ARG, "requests %u and %zu both move rows of page %u", owner, r, id);
+                // The requests run side by side: none may touch a page whose rows another one moves. Nor may a page stand twice in
+                // a table: a row could be read after it has been written under its other position.
+                if (owners.claim(id, pt_off[r] + at) != pt_off[r] + at)
+                    return ctx->fail(MLC_ERR_INVALID_ARG, "rows of page %u move in two places of the page tables, one of them request %zu's", id, r);
             }
             const uint64_t src_row = src_page * static_cast<uint64_t>(P) + from % P, dst_row = dst_page * static_cast<uint64_t>(P) + to % P;
             if ((src_row | dst_row) >> 32) return ctx->fail(MLC_ERR_UNSUPPORTED, "pool of 2^32 rows or more");

@@ -182,3 +182,14 @@ def test_pages_and_rows_beyond_four_gigabytes(ex):
     want[4:6] = moved.reshape(2, P, KVH, D)
     assert (pool[-8:].cpu().numpy() == want).all()
     assert (pool[0].cpu().numpy() == before[7]).all() and (pool[1] == 7).all()
+
+
+def test_a_page_twice_in_one_table_is_refused_where_rows_move(ex):
+    host, keep, ptrs = make_pools(9, 1, 4, 4, 2, 8, 2)
+    twice = [1, 1, 2]
+    assert not ex.compactKVRows(ptrs, twice, [0, 3], [0], [5, 6], [0, 2], 1, 4, 2, 8, 2, 4) and ex.last_status == 1
+    assert ex.compactKVRows(ptrs, twice, [0, 3], [8], [1, 2], [0, 2], 1, 4, 2, 8, 2, 4), "only page 2 has moving rows"
+    assert ex.compactKVRows(ptrs, twice, [0, 3], [0], [0, 1, 2, 3, 4, 5], [0, 6], 1, 4, 2, 8, 2, 4), "nothing moves"
+    want = host.copy()
+    want[:, 2, :2] = host[:, 2, 1:3]
+    assert (now(keep, 0, host.shape[1:]) == want).all()

@@ -6,8 +6,8 @@
 // counterpart; page and row layout are its (paged_kv.hpp:101-105).
 //
 // What bounds them: a call reads and writes every byte once, so the copy bandwidth of the memory for large calls (121 pages in
-// 64 pools, 2030 MB in and out: 254 us on the device) and one launch for small ones (three pages in 44 pools: 1.9 us on the
-// device, 5 with the host's part; rows of 32 requests in 64 pools, 20 MB: 4.3 and 12). That is why the pools' addresses and short id lists travel as kernel parameters: an upload in
+// 64 pools, 2030 MB in and out: 255 us on the device) and one launch for small ones (three pages in 44 pools: 1.9 us on the
+// device, 5 with the host's part; rows of 32 requests in 64 pools, 20 MB: 4.3 and 10). That is why the pools' addresses and short id lists travel as kernel parameters: an upload in
 // front of the kernel costs about as much as the kernel itself when a beam search copies a few pages.
 #include <algorithm>
 #include <cstring>
@@ -19,12 +19,15 @@ namespace mlcb {
 namespace {
 
 constexpr uint32_t kMaxPools = 128;      // per launch; a call with more takes several
-constexpr uint32_t kInlinePairs = 64;    // (source, destination) pairs that travel as kernel parameters; longer lists cost less uploaded
+// (source, destination) pairs that travel as kernel parameters: a kernel with few, since parameters cost the host's launch time, and
+// one with many (121 page pairs: 255.6 us, uploaded 259.7; 32 requests' rows: 9.9 us and 4.3 on the device, uploaded 11.9 and 9.5)
+constexpr uint32_t kFewPairs = 16, kManyPairs = 240;
 
+template <uint32_t INLINE>
 struct CopyParams {
     char* pools[kMaxPools];
     const uint2* pairs;                  // device list, or null: `inline_pairs`
-    uint2 inline_pairs[kInlinePairs];
+    uint2 inline_pairs[INLINE];
     uint64_t unit_bytes;                 // a page, or a row
     uint32_t n_pairs;
 };
@@ -33,8 +36,8 @@ constexpr uint32_t kBatch = 8;   // vectors a thread has in flight
 
 // Launched as a programmatic dependent of the kernel in front; it does not let its own dependents go before it is done, so
 // that nothing behind it reads a page early.
-template <typename Vec>
-__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams p, uint32_t chunks) {
+template <typename Vec, uint32_t INLINE>
+__global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__ CopyParams<INLINE> p, uint32_t chunks) {
     const uint32_t pair_i = blockIdx.x / chunks, chunk = blockIdx.x - pair_i * chunks;
     const uint2 pair = p.pairs ? p.pairs[pair_i] : p.inline_pairs[pair_i];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -56,18 +59,19 @@ __global__ void __launch_bounds__(256) copy_pages_kernel(const __grid_constant__
 // token order). A thread owns one column of the row in one pool and works through the request's moves in order, so a row
 // is always read before a later move can write it, whatever the other threads do. It has kBatch rows in flight: the rows it has not
 // read yet lie behind every destination of the batch.
+template <uint32_t INLINE>
 struct MoveParams {
     char* pools[kMaxPools];
     const uint2* moves;                  // device list, or null: `inline_moves`
     const uint32_t* first;               // [n_requests + 1] first move of a request, or null: `inline_first`
-    uint2 inline_moves[kInlinePairs];
-    uint32_t inline_first[kInlinePairs + 1];
+    uint2 inline_moves[INLINE];
+    uint32_t inline_first[INLINE + 1];
     uint64_t row_bytes;
     uint32_t n_requests;
 };
 
-template <typename Vec>
-__global__ void __launch_bounds__(128) move_rows_kernel(const __grid_constant__ MoveParams p, uint32_t vecs, uint64_t threads) {
+template <typename Vec, uint32_t INLINE>
+__global__ void __launch_bounds__(128) move_rows_kernel(const __grid_constant__ MoveParams<INLINE> p, uint32_t vecs, uint64_t threads) {
     const uint64_t id = static_cast<uint64_t>(blockIdx.x) * 128 + threadIdx.x;
     if (id >= threads) return;
     const uint32_t req = static_cast<uint32_t>(id / vecs), column = static_cast<uint32_t>(id - static_cast<uint64_t>(req) * vecs);
@@ -173,6 +177,82 @@ int wait_for_copy(mlc_ctx* ctx, const char* what) {
     return MLC_OK;
 }
 
+template <uint32_t INLINE>
+int launch_copies(mlc_ctx* ctx, void* const* pools, size_t n_pools, const uint32_t* src, const uint32_t* dst, size_t n_pairs,
+                  uint64_t page_bytes) {
+    std::vector<uint2> list;
+    CopyParams<INLINE> p{};
+    uint2* to = p.inline_pairs;
+    if (n_pairs > INLINE) {
+        list.resize(n_pairs);
+        to = list.data();
+    }
+    for (size_t i = 0; i < n_pairs; ++i) to[i] = make_uint2(src[i], dst[i]);
+    p.unit_bytes = page_bytes;
+    p.n_pairs = static_cast<uint32_t>(n_pairs);
+    const uint32_t vec = vector_bytes(pools, n_pools, page_bytes);
+    const uint64_t chunks = (page_bytes / vec + 256 * kBatch - 1) / (256 * kBatch);
+    if (chunks * n_pairs >= (uint64_t(1) << 31)) return ctx->fail(MLC_ERR_UNSUPPORTED, "too many pages in one call");
+    if (n_pairs > INLINE && !(p.pairs = static_cast<const uint2*>(stage_to_device(ctx, list.data(), n_pairs * sizeof(uint2)))))
+        return MLC_ERR_OOM;
+    for (size_t p0 = 0; p0 < n_pools; p0 += kMaxPools) {
+        const size_t n = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;
+        for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
+        const dim3 grid(static_cast<unsigned>(chunks * n_pairs), static_cast<unsigned>(n));
+        const uint32_t c = static_cast<uint32_t>(chunks);
+        cudaError_t e;
+        switch (vec) {
+            case 16: e = launch_dependent(ctx, copy_pages_kernel<uint4, INLINE>, grid, 256, 0, p, c); break;
+            case 8: e = launch_dependent(ctx, copy_pages_kernel<uint2, INLINE>, grid, 256, 0, p, c); break;
+            case 4: e = launch_dependent(ctx, copy_pages_kernel<uint32_t, INLINE>, grid, 256, 0, p, c); break;
+            default: e = launch_dependent(ctx, copy_pages_kernel<uint16_t, INLINE>, grid, 256, 0, p, c); break;
+        }
+        MLCB_CUDA(ctx, e);
+        ++ctx->launches;
+    }
+    return MLC_OK;
+}
+
+template <uint32_t INLINE>
+int launch_moves(mlc_ctx* ctx, void* const* pools, size_t n_pools, const std::vector<uint2>& moves, const std::vector<uint32_t>& first,
+                 uint64_t row_bytes) {
+    const size_t n_requests = first.size() - 1;
+    const uint32_t vec = vector_bytes(pools, n_pools, row_bytes);
+    const uint64_t vecs = row_bytes / vec, threads = vecs * n_requests;
+    if (vecs >> 32 || (threads + 127) / 128 >= (uint64_t(1) << 31)) return ctx->fail(MLC_ERR_UNSUPPORTED, "rows too long");
+    MoveParams<INLINE> p{};
+    if (moves.size() <= INLINE) {
+        std::memcpy(p.inline_moves, moves.data(), moves.size() * sizeof(uint2));
+        std::memcpy(p.inline_first, first.data(), first.size() * 4);
+    } else {
+        std::vector<uint32_t> image(moves.size() * 2 + first.size());
+        std::memcpy(image.data(), moves.data(), moves.size() * sizeof(uint2));
+        std::memcpy(image.data() + moves.size() * 2, first.data(), first.size() * 4);
+        const void* d = stage_to_device(ctx, image.data(), image.size() * 4);
+        if (!d) return MLC_ERR_OOM;
+        p.moves = static_cast<const uint2*>(d);
+        p.first = static_cast<const uint32_t*>(d) + moves.size() * 2;
+    }
+    p.row_bytes = row_bytes;
+    p.n_requests = static_cast<uint32_t>(n_requests);
+    for (size_t p0 = 0; p0 < n_pools; p0 += kMaxPools) {
+        const size_t n = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;
+        for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
+        const dim3 grid(static_cast<unsigned>((threads + 127) / 128), static_cast<unsigned>(n));
+        const uint32_t v = static_cast<uint32_t>(vecs);
+        cudaError_t e;
+        switch (vec) {
+            case 16: e = launch_dependent(ctx, move_rows_kernel<uint4, INLINE>, grid, 128, 0, p, v, threads); break;
+            case 8: e = launch_dependent(ctx, move_rows_kernel<uint2, INLINE>, grid, 128, 0, p, v, threads); break;
+            case 4: e = launch_dependent(ctx, move_rows_kernel<uint32_t, INLINE>, grid, 128, 0, p, v, threads); break;
+            default: e = launch_dependent(ctx, move_rows_kernel<uint16_t, INLINE>, grid, 128, 0, p, v, threads); break;
+        }
+        MLCB_CUDA(ctx, e);
+        ++ctx->launches;
+    }
+    return MLC_OK;
+}
+
 int copy_pages(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, const uint32_t* src, const uint32_t* dst,
                size_t n_pairs, size_t P, size_t KVH, size_t D, size_t dtype_bytes, size_t capacity_pages) {
     if (!ctx) return MLC_ERR_INVALID_ARG;
@@ -196,36 +276,9 @@ int copy_pages(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, cons
         if (src[i] != dst[i] && destinations.known(src[i]))
             return ctx->fail(MLC_ERR_INVALID_ARG, "page %u is a source and a destination", src[i]);
     DeviceGuard guard(ctx->device);
-    std::vector<uint2> list;
-    CopyParams p{};
-    uint2* to = p.inline_pairs;
-    if (n_pairs > kInlinePairs) {
-        list.resize(n_pairs);
-        to = list.data();
-    }
-    for (size_t i = 0; i < n_pairs; ++i) to[i] = make_uint2(src[i], dst[i]);
-    if (n_pairs > kInlinePairs && !(p.pairs = static_cast<const uint2*>(stage_to_device(ctx, list.data(), n_pairs * sizeof(uint2)))))
-        return MLC_ERR_OOM;
-    p.unit_bytes = page_bytes;
-    p.n_pairs = static_cast<uint32_t>(n_pairs);
-    const uint32_t vec = vector_bytes(pools, n_pools, page_bytes);
-    const uint64_t chunks = (page_bytes / vec + 256 * kBatch - 1) / (256 * kBatch);
-    if (chunks * n_pairs >= (uint64_t(1) << 31)) return ctx->fail(MLC_ERR_UNSUPPORTED, "too many pages in one call");
-    for (size_t p0 = 0; p0 < n_pools; p0 += kMaxPools) {
-        const size_t n = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;
-        for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
-        const dim3 grid(static_cast<unsigned>(chunks * n_pairs), static_cast<unsigned>(n));
-        const uint32_t c = static_cast<uint32_t>(chunks);
-        cudaError_t e;
-        switch (vec) {
-            case 16: e = launch_dependent(ctx, copy_pages_kernel<uint4>, grid, 256, 0, p, c); break;
-            case 8: e = launch_dependent(ctx, copy_pages_kernel<uint2>, grid, 256, 0, p, c); break;
-            case 4: e = launch_dependent(ctx, copy_pages_kernel<uint32_t>, grid, 256, 0, p, c); break;
-            default: e = launch_dependent(ctx, copy_pages_kernel<uint16_t>, grid, 256, 0, p, c); break;
-        }
-        MLCB_CUDA(ctx, e);
-        ++ctx->launches;
-    }
+    st = n_pairs <= kFewPairs ? launch_copies<kFewPairs>(ctx, pools, n_pools, src, dst, n_pairs, page_bytes)
+                              : launch_copies<kManyPairs>(ctx, pools, n_pools, src, dst, n_pairs, page_bytes);
+    if (st != MLC_OK) return st;
     note_pool_writes(ctx, pools, n_pools);
     return sync ? wait_for_copy(ctx, "page copy") : MLC_OK;
 }
@@ -280,41 +333,10 @@ int compact_rows(mlc_ctx* ctx, bool sync, void* const* pools, size_t n_pools, co
         if (moves.size() > first.back()) first.push_back(static_cast<uint32_t>(moves.size()));
     }
     if (moves.empty()) return MLC_OK;
-    const size_t n_requests = first.size() - 1;
     DeviceGuard guard(ctx->device);
-    MoveParams p{};
-    if (moves.size() <= kInlinePairs) {
-        std::memcpy(p.inline_moves, moves.data(), moves.size() * sizeof(uint2));
-        std::memcpy(p.inline_first, first.data(), first.size() * 4);
-    } else {
-        std::vector<uint32_t> image(moves.size() * 2 + first.size());
-        std::memcpy(image.data(), moves.data(), moves.size() * sizeof(uint2));
-        std::memcpy(image.data() + moves.size() * 2, first.data(), first.size() * 4);
-        const void* d = stage_to_device(ctx, image.data(), image.size() * 4);
-        if (!d) return MLC_ERR_OOM;
-        p.moves = static_cast<const uint2*>(d);
-        p.first = static_cast<const uint32_t*>(d) + moves.size() * 2;
-    }
-    p.row_bytes = row_bytes;
-    p.n_requests = static_cast<uint32_t>(n_requests);
-    const uint32_t vec = vector_bytes(pools, n_pools, row_bytes);
-    const uint64_t vecs = row_bytes / vec, threads = vecs * n_requests;
-    if (vecs >> 32 || (threads + 127) / 128 >= (uint64_t(1) << 31)) return ctx->fail(MLC_ERR_UNSUPPORTED, "rows too long");
-    for (size_t p0 = 0; p0 < n_pools; p0 += kMaxPools) {
-        const size_t n = n_pools - p0 < kMaxPools ? n_pools - p0 : kMaxPools;
-        for (size_t i = 0; i < n; ++i) p.pools[i] = static_cast<char*>(pools[p0 + i]);
-        const dim3 grid(static_cast<unsigned>((threads + 127) / 128), static_cast<unsigned>(n));
-        const uint32_t v = static_cast<uint32_t>(vecs);
-        cudaError_t e;
-        switch (vec) {
-            case 16: e = launch_dependent(ctx, move_rows_kernel<uint4>, grid, 128, 0, p, v, threads); break;
-            case 8: e = launch_dependent(ctx, move_rows_kernel<uint2>, grid, 128, 0, p, v, threads); break;
-            case 4: e = launch_dependent(ctx, move_rows_kernel<uint32_t>, grid, 128, 0, p, v, threads); break;
-            default: e = launch_dependent(ctx, move_rows_kernel<uint16_t>, grid, 128, 0, p, v, threads); break;
-        }
-        MLCB_CUDA(ctx, e);
-        ++ctx->launches;
-    }
+    st = moves.size() <= kFewPairs ? launch_moves<kFewPairs>(ctx, pools, n_pools, moves, first, row_bytes)
+                                   : launch_moves<kManyPairs>(ctx, pools, n_pools, moves, first, row_bytes);
+    if (st != MLC_OK) return st;
     note_pool_writes(ctx, pools, n_pools);
     return sync ? wait_for_copy(ctx, "row compaction") : MLC_OK;
 }

@@ -125,6 +125,7 @@ int check_tables(TreeShape& s, const TreeTables& t, size_t n_flat, std::string* 
     if (s.batch == 0 || s.H == 0 || s.D == 0 || s.P == 0) return no(MLC_ERR_INVALID_ARG, "zero dimension");
     if (s.KVH == 0 || s.H % s.KVH != 0) return no(MLC_ERR_INVALID_ARG, "num_heads must be a multiple of kv_heads");
     if (s.D > 256) return no(MLC_ERR_UNSUPPORTED, "head_dim > 256");
+    if (s.P >= (size_t(1) << 31) || s.mask_words > (size_t(1) << 27)) return no(MLC_ERR_UNSUPPORTED, "page_size_tokens or mask_words too large");
     if (!t.pt_off || !t.prefix || !t.draft || (!t.pt_flat && n_flat)) return no(MLC_ERR_INVALID_ARG, "null table");
     for (size_t r = 0; r < s.batch; ++r)
         if (t.pt_off[r + 1] < t.pt_off[r]) return no(MLC_ERR_BOUNDS, "page_table_offsets not monotone at %zu", r);
@@ -155,6 +156,9 @@ int check_call(mlc_ctx* ctx, const TreeArgs& a) {
     if (!a.q || !a.k_pages || !a.v_pages || !a.o) return ctx->fail(MLC_ERR_INVALID_ARG, "null buffer");
     if ((a.q_dtype != MLC_F32 && a.q_dtype != MLC_F16) || (a.o_dtype != MLC_F32 && a.o_dtype != MLC_F16))
         return ctx->fail(MLC_ERR_INVALID_ARG, "q / o dtype must be MLC_F16 or MLC_F32");
+    if (!aligned_to(a.q, a.q_dtype == MLC_F32 ? 4 : 2) || !aligned_to(a.o, a.o_dtype == MLC_F32 ? 4 : 2) || !aligned_to(a.k_pages, 2) ||
+        !aligned_to(a.v_pages, 2))
+        return ctx->fail(MLC_ERR_INVALID_ARG, "buffers must be aligned to their elements");
     return MLC_OK;
 }
 

@@ -111,7 +111,7 @@ paged_tree_general_kernel(const QT* __restrict__ q, const __half* __restrict__ k
 
 int launch_tree_general(mlc_ctx* ctx, const TreeShape& s, const TreeView& v, const TreeArgs& a) {
     const dim3 grid(static_cast<unsigned>(s.tokens * s.H)), block(kWarps * 32);
-    const uint32_t cap32 = s.capacity ? static_cast<uint32_t>(s.capacity) : 0xFFFFFFFFu;
+    const uint32_t cap32 = s.capacity && s.capacity < 0xFFFFFFFFu ? static_cast<uint32_t>(s.capacity) : 0xFFFFFFFFu;
     auto kp = static_cast<const __half*>(a.k_pages);
     auto vp = static_cast<const __half*>(a.v_pages);
 #define MLCB_TREE_LAUNCH(QT, OT)                                                                                       \

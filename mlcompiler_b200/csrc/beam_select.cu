@@ -147,7 +147,8 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
         for (uint32_t i = lane; i < p.segments; i += 32) {   // a segment of -inf alone has the sum 0
             const float2 v = __ldcg(sums + i);
             const float both = fmaxf(m, v.x);
-            if (both > -INFINITY) s = s * static_cast<double>(exp_diff(m, both)) + static_cast<double>(v.y) * static_cast<double>(exp_diff(v.x, both));
+            if (both > -INFINITY)
+                s = s * static_cast<double>(exp_diff(m, both)) + static_cast<double>(v.y) * static_cast<double>(exp_diff(v.x, both));
             m = both;
         }
         float all = m;
@@ -171,7 +172,8 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
         } else {
             const uint32_t b = i / p.segments;
             if (c >= p.n_select || (p.finished && p.finished[row0 + b])) return false;
-            const uint64_t key = i == tid && c == 0 ? head_key : __ldcg(&p.keys[(static_cast<size_t>(row0) * p.segments + i) * p.n_select + c]);
+            const uint64_t key = i == tid && c == 0
+                                     ? head_key : __ldcg(&p.keys[(static_cast<size_t>(row0) * p.segments + i) * p.n_select + c]);
             if (key == 0) return false;
             got = {static_cast<double>(p.cum[row0 + b]) + (static_cast<double>(key_value(key)) - sh.lse[b]), b, key_token(key)};
         }
@@ -184,7 +186,8 @@ __device__ __noinline__ void join_group(const BeamParams& p, Shared& sh, uint32_
     for (uint32_t i = tid; i < lists * deep + p.beams; i += kThreads) {
         const uint32_t d = i / lists;
         Candidate c;
-        if (d < deep ? candidate(i - d * lists, d, c) : candidate(i - lists * deep + lists, 0, c)) top = fmaxf(top, __double2float_rd(c.score));
+        if (d < deep ? candidate(i - d * lists, d, c) : candidate(i - lists * deep + lists, 0, c))
+            top = fmaxf(top, __double2float_rd(c.score));
     }
     sh.tops[tid] = top;
     __syncthreads();
@@ -466,7 +469,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) beam_select_kernel(const
     const uint32_t unit = warp * p.ctas_per_group + (blockIdx.x - group * p.ctas_per_group);
     if (unit < p.beams * p.segments) {
         const uint32_t row = group * p.beams + unit / p.segments;
-        if (!p.finished || !p.finished[row]) segment(p, sh.ring[warp], sh.list[warp], &sh.listed[warp], sh.part[warp], row, unit % p.segments, lane);
+        if (!p.finished || !p.finished[row])
+            segment(p, sh.ring[warp], sh.list[warp], &sh.listed[warp], sh.part[warp], row, unit % p.segments, lane);
     }
     // the last CTA of the group joins: thread 0 publishes what the CTA wrote, and sees what the others published
     __syncthreads();

@@ -404,3 +404,41 @@ def test_pages_beyond_four_gigabytes(ex, D, KVH):
                                     64, 0.0, F16, F16, capacity), ex.last_error()
     assert ex.lastAttentionKernel() == (4 if D == 64 else 1)
     check(case, dev, dev.result(case))
+
+
+@pytest.mark.parametrize("D", [64, 20])
+def test_buffers_off_their_alignment(ex, D):
+    """Off 16 bytes is the general kernel's; off an element is refused on the host."""
+    import torch
+    case = TreeCase(77, [70, 3], [5, 2], 4, 2, D)
+    dev = OnDevice(case)
+    tables = (*case.tables(), case.N, 4, 2, D, 64, 0.0, F16, F16, case.capacity)
+    q, k, v, o = (t.data_ptr() for t in (dev.q, dev.k, dev.v, dev.o))
+    for bad in ((q + 1, k, v, o), (q, k + 1, v, o), (q, k, v + 1, o), (q, k, v, o + 1)):
+        assert not ex.runPagedTreeAttention(*bad, *tables) and ex.last_status == 1
+    shifted = []
+    for t in (dev.q, dev.k, dev.v):
+        wide = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        wide[1:] = t.reshape(-1)
+        shifted.append(wide)
+    torch.cuda.synchronize()
+    assert ex.runPagedTreeAttention(*(t.data_ptr() + 2 for t in shifted), o, *tables), ex.last_error()
+    assert ex.lastAttentionKernel() == 1
+    check(case, dev, dev.result(case))
+
+
+def test_sizes_beyond_the_kernels_types_are_refused(ex):
+    case = TreeCase(78, [70], [5], 4, 2, 64)
+    dev = OnDevice(case)
+    for P, words in (((1 << 32) + 64, None), (1 << 62, None), (1 << 31, None), (64, (1 << 27) + 1)):
+        flat, off, prefix, draft, mask = case.tables()
+        if words:   # the size alone is looked at
+            t = capi.Executor._treeTables(flat, off, prefix, draft, mask, 1)
+            args = list(t[1])
+            args[-1] = words
+            status = ex._lib.mlc_run_paged_tree_attention(ex._h, dev.q.data_ptr(), dev.k.data_ptr(), dev.v.data_ptr(), dev.o.data_ptr(), *args,
+                                                          1, 4, 2, 64, P, 0.0, F16, F16, case.capacity)
+            assert status == 5
+        else:
+            assert not ex.runPagedTreeAttention(dev.q, dev.k, dev.v, dev.o, flat, off, prefix, draft, mask, 1, 4, 2, 64, P, 0.0, F16, F16,
+                                                case.capacity) and ex.last_status == 5

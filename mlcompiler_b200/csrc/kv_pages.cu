@@ -6,9 +6,10 @@
 // counterpart; page and row layout are its (paged_kv.hpp:101-105).
 //
 // What bounds them: a call reads and writes every byte once, so the copy bandwidth of the memory for large calls (121 pages
-// from 80 different ones in 64 pools, 1690 MB in and out: 255 us on the device) and one launch for small ones (three pages in 44 pools: 1.9 us on the
-// device, 5 with the host's part; rows of 32 requests in 64 pools, 20 MB: 4.3 and 10). That is why the pools' addresses and
-// short id lists travel as kernel parameters: an upload in front of the kernel costs about as much as the kernel itself.
+// from 80 different ones in 64 pools, 1690 MB in and out: 255 us on the device) and one launch for small ones (three pages in
+// 44 pools: 1.9 us on the device, 5 with the host's part; rows of 32 requests in 64 pools, 20 MB: 4.3 and 10). That is why the
+// pools' addresses and short id lists travel as kernel parameters: an upload in front of the kernel costs about as much as the
+// kernel itself.
 #include <algorithm>
 #include <cstring>
 

@@ -388,8 +388,9 @@ __device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kSte
         const float top = four_maxima(x, quarter);
         add_step(x, top, m, s);
         if (step == 0) {   // 64 disjoint parts: at least n_select logits reach the n_select-th largest of their maxima
-            part[lane] = fmaxf(quarter[0], quarter[1]);
-            part[lane + 32] = fmaxf(quarter[2], quarter[3]);
+            // (a part of NaN alone counts as -inf: NaN is never above anything, and the lanes would not agree on a threshold)
+            part[lane] = max3(quarter[0], quarter[1], -INFINITY);
+            part[lane + 32] = max3(quarter[2], quarter[3], -INFINITY);
             __syncwarp();
             threshold = fmaxf(kLowest, kth_of_64(part, p.n_select, lane));
         }

@@ -282,3 +282,32 @@ def test_logits_beyond_four_gigabytes(ex):
     # two factors that bring lane and row to one maximum. The score is rounded once.
     tol = (528 + 4 + 3 * 9) * 2.0**-24 + 2.0**-24 * np.abs(want).max()
     assert np.abs(dev[1].cpu().numpy() - want).max() <= tol
+
+
+def mostly_nan(seed, V, kept):
+    """One row of NaN with numbers at `kept` only, in a random order of size."""
+    x = np.full(V, np.nan, np.float32)
+    x[kept] = np.random.default_rng(seed).permutation(len(kept)) * 0.25 - 3.0
+    return x
+
+
+@pytest.mark.parametrize("n", [1, 2, 4, 8, 40])
+@pytest.mark.parametrize("V", [512, 513, 1500, 40000])
+def test_rows_of_mostly_nan(ex, n, V):
+    """NaN counts as -inf also where it leaves a lane of the first step no number, and where a few numbers are all there is."""
+    rng = np.random.default_rng(50)
+    rows = [mostly_nan(0, V, np.arange(4)), mostly_nan(1, V, np.arange(V - 5, V)),
+            mostly_nan(2, V, np.arange(0, V, 37)), mostly_nan(3, V, np.arange(272, 276))]
+    rows += [mostly_nan(4 + i, V, np.flatnonzero(rng.random(V) < 0.2)) for i in range(12)]
+    for i, (start, count) in enumerate([(0, 132), (4, 132), (100, 200), (0, 480), (16, 400), (0, 508)]):   # runs of NaN
+        x = (rng.standard_normal(V) * 2.5).astype(np.float32)
+        x[start: start + count] = np.nan
+        rows.append(x)
+    x = (rng.standard_normal(V) * 2.5).astype(np.float32)
+    x[[0, 1, 2, 3, 128, 129, 130, 131]] = np.nan                 # all that a lane takes for its first part
+    rows += [x, np.where(np.arange(V) == 272, 10, np.where(np.arange(V) == 273, 9, x)).astype(np.float32)]
+    x = np.stack(rows)
+    cum = np.zeros((len(rows), 1), np.float32)
+    check(run(ex, x, cum, None, n), reference(x, cum, None, n, 0))
+    cum = -np.arange(len(rows), dtype=np.float32).reshape(-1, 2) * 0.015625
+    check(run(ex, x, cum, None, n), reference(x, cum, None, n, 0))

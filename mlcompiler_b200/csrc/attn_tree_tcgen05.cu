@@ -6,8 +6,10 @@
 // them. Per 64 tokens of the cache:
 //   S[128x64]  = Q[128xD] . K^T       A and B from shared memory, fp32 accumulator in tensor memory
 //   softmax    : thread t owns row t; reference maximum and sum in fp32, base-2 exponentials, P rounded to fp16 back into
-//                tensor memory as the next A operand. The reference is the maximum of the run's first tile and moves up
-//                only when the weights outgrow fp16 (exact: the final 1 / l uses the same reference)
+//                tensor memory as the next A operand: 2^-11 of each weight at most, as much as the result's own rounding. The
+//                reference is the maximum of the run's first tile and moves up only when the weights outgrow fp16 (exact: the
+//                final 1 / l uses the same reference). Its weight is 2^8: fp16 has 15 powers of two above 1 and loses bits
+//                below 2^-14, which beside one dominant token is where all others lie; 64 equal weights sum to half the limit
 //   O[128xD] += P[128x64] . V
 // The tree mask only matters in the tiles that hold drafted tokens, the last ones of a request: there a row's 64 mask
 // bits are cut out of its mask words. In those tiles V is also searched for infinities and NaN - a masked token has
@@ -15,8 +17,11 @@
 // that do see them.
 //
 // fp32 queries or outputs (EXACT): an fp16 operand carries 11 bits, so Q (scaled by a power of two per row) and P enter as
-// two fp16 halves, two products each: 22 bits of each, K and V are fp16 as they are. The products of a tile are added to
-// those before it outside the tensor core.
+// two fp16 halves, two products each; K and V are fp16 as they are. The products of a tile are added to those before it
+// outside the tensor core, so every tile has a reference of its own, its maximum, with a weight of 2^15: 22 bits of a weight
+// down to 2^-18 of the tile's largest, 2^-40 of the largest below. With one token 9 or 15 nats above 600 equal ones, and of
+// value 0, the result is off by 7e-7 and 2e-7 of its size; with the first tile's maximum at 1 it was 2e-4 and 2e-2. (8 requests
+// in fp32: 19.1 us, 18.8 with the shared reference.)
 //
 // What bounds it: the cache is read once, 4 * rows flop per byte - memory up to about 128 rows, the exponentials and the
 // tensor core's issue above. The cache tiles of all (request, KV head, row tile) units are dealt evenly to a resident
@@ -41,6 +46,8 @@ constexpr uint32_t kSlabKV = kTreeTile * 128;  // 64 halfs of every token of a t
 constexpr uint32_t kThreads = 256;   // two whole warpgroups, for the register split; warp 7 has no work
 constexpr uint32_t kRegsSoftmax = 168, kRegsOther = 88;   // registers a thread of the two warpgroups, where they are split
 constexpr uint32_t kStageBytes = 32 * 128;     // per softmax warp: 128 bytes of each of its rows, on the way in or out
+// Exponent of the reference's weight, and where the sum of a tile's weights has outgrown it (each is below the sum)
+constexpr float kRefLog2 = 8.f, kRefLog2Exact = 15.f, kSumLimit = 32768.f;
 
 template <int D, bool EXACT>
 struct Config {
@@ -72,7 +79,7 @@ struct TreeParams {
     const __half* v_pages;
     void* o;
     float* part_o;    // [slot][slot_rows][D]
-    float2* part_ml;  // [slot][slot_rows] (reference maximum in base-2 units, sum)
+    float2* part_ml;  // [slot][slot_rows] (exponent that takes the part to a common scale, sum)
     const TreePiece* pieces;
     const uint32_t *pt_flat, *mask;
     uint32_t* err;
@@ -344,7 +351,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     };
 
     // Two fp32 CTAs an SM leave a thread 128 registers at launch, and softmax with both halves of P spills: the other warpgroup
-    // gives it some (the sum stays 2 * 128). 8 requests in fp32: 20.3 us without, 19.4 with; fp16 does not gain.
+    // gives it some (the sum stays 2 * 128). 8 requests in fp32, with one reference for all tiles: 20.3 us without, 19.4 with; fp16 does not gain.
     if constexpr (EXACT && C::ctas == 2) {
         if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -506,7 +513,10 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
             const uint32_t r = p.row_begin + min(row, p.n_rows - 1);
             const uint32_t* mask = prm.mask + static_cast<size_t>(p.token0 + r / prm.G) * prm.mask_words;
             const float scale = prm.scale_log2 * row_down;      // of a raw score, base-2 units
-            float m_ref = -INFINITY, l_sum = 0.f;               // reference maximum (raw scores) of the accumulator, row sum
+            // A weight is 2^(score * scale + offset), the offset that of the accumulator's reference; infinite: nothing seen yet.
+            // It is this rounded number that all factors are taken from, so that its rounding cancels.
+            float m_ref = -INFINITY, offset = INFINITY, l_sum = 0.f;   // reference maximum (raw scores), row sum
+            float o_factor = 1.0f;                              // EXACT: of the last tile's products, to the reference
             for (uint32_t j = 0; j < p.n_tiles; ++j, ++g) {
                 const uint32_t kv0 = (p.tile_begin + j) * kTreeTile;
                 where = 0x20;
@@ -517,11 +527,8 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                     const uint32_t tS = tmem + lane_base + C::tmem_s + (g & 1u) * kTreeTile;
                     uint32_t hi[32], lo[EXACT ? 32 : 1];
                     float alpha = 1.0f;
-                    // First with the reference maximum as it is, without looking for the tile's: every weight is below the
-                    // row's sum over the tile, and while that is below 2^15 the weights fit fp16. Where some row's sum is not
-                    // (or is NaN), and on a run's first tile, the tile is done (again) with a new reference.
-                    for (bool moved = j == 0;; moved = true) {
-                        uint32_t s[64];
+                    uint32_t s[64];
+                    auto load_scores = [&] {
                         {
                             uint32_t a[32], b[32];
                             tc::tmem_ld32(tS, a);
@@ -548,23 +555,20 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                                 if (!((see_hi >> c) & 1u)) s[32 + c] = 0xff800000u;
                             }
                         }
-                        if (moved) {
-                            float top = m_ref;   // fmaxf passes over NaN
+                    };
+                    auto largest = [&](float top) {   // fmaxf passes over NaN
 #pragma unroll
-                            for (int c = 0; c < 64; ++c) top = fmaxf(top, __uint_as_float(s[c]));
-                            if (top > m_ref) {
-                                alpha = m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * scale);
-                                m_ref = top;
-                            }
-                            l_sum *= alpha;
-                        }
-                        const float neg_m = m_ref == -INFINITY ? 0.f : -m_ref * scale;
-                        const float2 scale2 = make_float2(scale, scale), neg_m2 = make_float2(neg_m, neg_m);
+                        for (int c = 0; c < 64; ++c) top = fmaxf(top, __uint_as_float(s[c]));
+                        return top;
+                    };
+                    auto weights = [&](float from) {   // into hi (and lo); returns their sum
+                        const float add = from == INFINITY ? 0.f : from;
+                        const float2 scale2 = make_float2(scale, scale), add2s = make_float2(add, add);
                         float2 ps[2] = {};
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
                             const float2 raw = make_float2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-                            float2 x = fma2(raw, scale2, neg_m2);
+                            float2 x = fma2(raw, scale2, add2s);
                             x = make_float2(ex2(x.x), ex2(x.y));
                             ps[i & 1] = add2(ps[i & 1], x);
                             const __half2 h = __float22half2_rn(x);
@@ -575,27 +579,56 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                             }
                         }
                         ps[0] = add2(ps[0], ps[1]);
-                        const float sum = ps[0].x + ps[0].y;
-                        if (!moved) {
-                            // (a reference of -inf is none)
-                            if (__any_sync(0xffffffffu, !(sum < 32768.0f) || m_ref == -INFINITY)) continue;
-                        } else if (!EXACT && j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-                            where = 0x21;
-                            ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
-                            if (!ok) break;
-                            tc::fence_after();
-#pragma unroll 1
-                            for (int c0 = 0; c0 < D; c0 += 32) {
-                                uint32_t o[32];
-                                tc::tmem_ld32(tmem + lane_base + c0, o);
-                                tc::tmem_wait_ld();
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                                tmem_st32(tmem + lane_base + c0, o);
+                        return ps[0].x + ps[0].y;
+                    };
+                    float before_factor = 1.0f;   // EXACT: o_factor of the tile before
+                    if constexpr (EXACT) {
+                        load_scores();
+                        const float top = largest(-INFINITY);
+                        const float own = top == -INFINITY ? INFINITY : fmaf(-top, scale, kRefLog2Exact);
+                        const float both = fminf(offset, own);
+                        alpha = offset == INFINITY ? 0.f : ex2(both - offset);
+                        before_factor = o_factor;
+                        o_factor = own == INFINITY ? 0.f : ex2(both - own);
+                        offset = both;
+                        l_sum = l_sum * alpha + weights(own) * o_factor;
+                    } else {
+                        // First with the reference as it is, without looking for the tile's maximum: every weight is below the row's
+                        // sum over the tile, and while that is below the limit the weights fit fp16. Where some row's sum is not
+                        // (or is NaN), and on a run's first tile, the tile is done (again) with a new reference.
+                        for (bool moved = j == 0;; moved = true) {
+                            load_scores();
+                            if (moved) {
+                                const float top = largest(m_ref);
+                                if (top > m_ref) {
+                                    const float from = fmaf(-top, scale, kRefLog2);
+                                    alpha = m_ref == -INFINITY ? 0.f : ex2(from - offset);
+                                    m_ref = top;
+                                    offset = from;
+                                }
+                                l_sum *= alpha;
                             }
+                            const float sum = weights(offset);
+                            if (!moved) {
+                                if (__any_sync(0xffffffffu, !(sum < kSumLimit) || offset == INFINITY)) continue;
+                            } else if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+                                where = 0x21;
+                                ok = warp_wait(smem_u32(&bars.pv_done), (g - 1) & 1u);   // O may only be touched once P.V is done
+                                if (!ok) break;
+                                tc::fence_after();
+#pragma unroll 1
+                                for (int c0 = 0; c0 < D; c0 += 32) {
+                                    uint32_t o[32];
+                                    tc::tmem_ld32(tmem + lane_base + c0, o);
+                                    tc::tmem_wait_ld();
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                                    tmem_st32(tmem + lane_base + c0, o);
+                                }
+                            }
+                            l_sum += sum;
+                            break;
                         }
-                        l_sum += sum;
-                        break;
                     }
                     if (!ok) break;
                     // P over this tile's scores (own lane, already read): the halves in 32 columns each
@@ -619,7 +652,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) {
                                     const float before = j > 1 ? __uint_as_float(sum[i]) : 0.f;
-                                    sum[i] = __float_as_uint((before + __uint_as_float(o[i])) * alpha);
+                                    sum[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), before_factor, before) * alpha);
                                 }
                                 tmem_st32(tmem + lane_base + C::tmem_sum + c0, sum);
                             }
@@ -686,7 +719,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                 const size_t out = (static_cast<size_t>(done.token0 + r / prm.G) * prm.H + done.kv_head * prm.G + r % prm.G) * D;
                 const size_t part = static_cast<size_t>(done.slot) * prm.slot_rows + row;
                 const bool repair = *reinterpret_cast<volatile uint32_t*>(&bars.not_finite[pi & 1u]) == pi + 1;
-                if (!whole && mine) prm.part_ml[part] = make_float2(m_ref == -INFINITY ? -INFINITY : m_ref * scale, l_sum);
+                if (!whole && mine) prm.part_ml[part] = make_float2(-offset, l_sum);
                 // drafted tokens of this piece that the row sees: what is not finite in V belongs in its output
                 auto put_back = [&](int c0, uint32_t (&o)[32]) {
                     const uint32_t begin = done.tile_begin * kTreeTile, stop = min(len, begin + done.n_tiles * kTreeTile);
@@ -717,7 +750,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
                             tc::tmem_ld32(tmem + lane_base + C::tmem_sum + c0 + 32 * half, sum);
                             tc::tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(sum[i]) + __uint_as_float(o[i]));
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(__uint_as_float(o[i]), o_factor, __uint_as_float(sum[i])));
                         }
                         if (repair && mine) put_back(c0 + 32 * half, o);
 #pragma unroll

@@ -687,7 +687,7 @@ void mlc_page_pool_destroy(mlc_page_pool* pool);
 int mlc_page_pool_allocate(mlc_page_pool* pool, uint32_t* page_id);
 int mlc_page_pool_allocate_n(mlc_page_pool* pool, size_t n, uint32_t* out /* [n] */);
 /* release: the reference asserts on a bad id (paged_kv.cpp:37-42); this returns 0 and
- * changes nothing. */
+ * changes nothing, for a page that is free already too. */
 int mlc_page_pool_release(mlc_page_pool* pool, uint32_t page_id);
 /* Shared pages (no counterpart in the reference, whose pages have one owner). share adds an owner to a page in
  * use (0 if it is not); release takes one away, and frees the page with the last. owners: 0 = free. */

@@ -33,7 +33,7 @@ bool PagePool::allocate_n(size_t n, std::vector<uint32_t>& out) {
 }
 
 bool PagePool::release(uint32_t page_id) {
-    if (page_id >= capacity_ || in_use_ == 0) return false;
+    if (page_id >= capacity_ || owners_[page_id] == 0) return false;
     if (owners_[page_id] > 1) {
         --owners_[page_id];
         return true;

@@ -26,7 +26,7 @@ public:
     std::optional<uint32_t> allocate();
     // All or nothing: appends n ids to `out`, or leaves pool and `out` untouched.
     bool allocate_n(size_t n, std::vector<uint32_t>& out);
-    // Returns false (and changes nothing) for an id outside the pool or with nothing in use;
+    // Returns false (and changes nothing) for an id outside the pool or of a page that is free;
     // the reference asserts in debug builds and is undefined in release builds.
     // A page with several owners (see share) loses one of them and stays in use.
     bool release(uint32_t page_id);

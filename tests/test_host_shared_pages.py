@@ -125,3 +125,13 @@ def test_random_forks_against_a_model():
                 listed[p] = listed.get(p, 0) + 1
         assert all(pool.owners(p) == listed.get(p, 0) for p in range(40))
         assert pool.pages_in_use() == len(listed) and pool.pages_in_use() + pool.pages_free() == 40
+
+
+def test_a_free_page_is_not_released_again():
+    pool = PagePool(4)
+    a, b = pool.allocate(), pool.allocate()
+    assert pool.release(a)
+    assert not pool.release(a) and not pool.release(3)  # free, and never handed out
+    assert pool.pages_in_use() == 1 and pool.pages_free() == 3 and pool.owners(b) == 1
+    got = [pool.allocate() for _ in range(3)]
+    assert sorted(got + [b]) == [0, 1, 2, 3] and pool.allocate() is None

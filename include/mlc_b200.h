@@ -707,11 +707,14 @@ int mlc_kv_state_extend_one_token(mlc_kv_state* state, mlc_page_pool* pool, uint
 /* Several continuations of one request. fork: `state`, which has no pages, becomes a second owner of all of
  * `parent`'s. extend_one_token fails where it would write into a page with other owners; the _owned form takes a
  * new page in its place and returns 2 with the copy that is owed before anything is written there (copy_dst
- * becomes a copy of copy_src: mlc_encode_copy_kv_pages), 1 if none is, 0 on failure. truncate keeps the first
+ * becomes a copy of copy_src: mlc_encode_copy_kv_pages), 1 if none is, 0 on failure. undo_copy is for a copy that
+ * could not be made: the state names copy_src again, as one of its owners, and copy_dst is free; the tokens stay
+ * counted (truncate takes them back). 0 if the state does not name copy_dst or copy_src is free. truncate keeps the first
  * `tokens` tokens and releases the pages behind them (0 if there are fewer tokens): what a rejected draft took. */
 int mlc_kv_state_fork(mlc_kv_state* state, const mlc_kv_state* parent, mlc_page_pool* pool);
 int mlc_kv_state_extend_one_token_owned(mlc_kv_state* state, mlc_page_pool* pool, uint32_t* page_id, uint32_t* slot_in_page,
                                         uint32_t* copy_src, uint32_t* copy_dst);
+int mlc_kv_state_undo_copy(mlc_kv_state* state, mlc_page_pool* pool, uint32_t copy_src, uint32_t copy_dst);
 int mlc_kv_state_truncate(mlc_kv_state* state, mlc_page_pool* pool, size_t tokens);
 int mlc_kv_state_locate(const mlc_kv_state* state, size_t pos, uint32_t* page_id, uint32_t* slot_in_page);
 void mlc_kv_state_release_all(mlc_kv_state* state, mlc_page_pool* pool);

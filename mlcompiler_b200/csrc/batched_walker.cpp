@@ -45,7 +45,7 @@ static double now_us() {
     return std::chrono::duration<double, std::micro>(std::chrono::steady_clock::now().time_since_epoch()).count();
 }
 
-bool BatchedWalker::copy_shared_pages(const PageCopies& copies) {
+bool BatchedWalker::copy_shared_pages(const PageCopies& copies, const std::vector<RequestKVState*>& states) {
     if (copies.empty()) return true;
     PagedAttentionExecutor& ex = exec_;
     const PagedKVStorage* storage = ex.storage_;
@@ -60,10 +60,15 @@ bool BatchedWalker::copy_shared_pages(const PageCopies& copies) {
         copy_src_.push_back(c.first);
         copy_dst_.push_back(c.second);
     }
-    return mlc_pass_begin(ex.ctx_) == MLC_OK &&
-           mlc_encode_copy_kv_pages(ex.ctx_, copy_pools_.data(), copy_pools_.size(), copy_src_.data(), copy_dst_.data(), copies.size(),
-                                    storage->page_size_tokens(), storage->n_kv_heads(), storage->head_dim(), storage->dtype_bytes(),
-                                    storage->capacity_pages()) == MLC_OK;
+    if (mlc_pass_begin(ex.ctx_) == MLC_OK &&
+        mlc_encode_copy_kv_pages(ex.ctx_, copy_pools_.data(), copy_pools_.size(), copy_src_.data(), copy_dst_.data(), copies.size(),
+                                 storage->page_size_tokens(), storage->n_kv_heads(), storage->head_dim(), storage->dtype_bytes(),
+                                 storage->capacity_pages()) == MLC_OK)
+        return true;
+    for (auto c = copies.rbegin(); c != copies.rend(); ++c)
+        for (RequestKVState* s : states)
+            if (s && s->undo_copy(*ex.pool_, c->first, c->second)) break;
+    return false;
 }
 
 BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, const LogitsSink* sink,
@@ -78,10 +83,15 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
     const size_t N = slots.size();
     const uint32_t H = ex.H_, KVH = ex.KVH_, D = ex.D_, P = storage->page_size_tokens();
     PageCopies copies;
-    bool copied = false;
+    std::vector<RequestKVState*> states(N, nullptr);
+    bool copied = false;   // or taken back
+    auto make_copies = [&] {
+        copied = true;
+        return copy_shared_pages(copies, states);
+    };
     auto fail_all = [&]() {
         // a page table already names the copies: they are made even if the pass is not
-        if (!copied) copied = copy_shared_pages(copies);
+        if (!copied) make_copies();
         if (!copies.empty()) mlc_pass_flush(ctx);
         out.per_request.clear();
         for (const auto& s : slots) {
@@ -104,16 +114,14 @@ BatchedDecodeOutput BatchedWalker::step(const std::vector<RequestSlot>& slots, c
             reqs[r]->page_state->request_id = slots[r].request_id;
             reqs[r]->page_state->page_size_tokens = ex.page_size_tokens_;
         }
-        auto loc = reqs[r]->page_state->extend_one_token(*ex.pool_, &copies);
+        states[r] = reqs[r]->page_state.get();
+        auto loc = states[r]->extend_one_token(*ex.pool_, &copies);
         if (!loc) return fail_all();
         page_ids[r] = loc->first;
         slot_ids[r] = loc->second;
     }
 
-    if (!(copied = copy_shared_pages(copies))) {
-        copied = true;   // not a second time
-        return fail_all();
-    }
+    if (!make_copies()) return fail_all();
 
     // Tables of the pass, built once (the reference rebuilds them per layer, 316-325):
     // seq_lens count the new token, q_pos is the new token's own position.
@@ -522,7 +530,9 @@ std::vector<float> BatchedWalker::prefill_model(uint32_t request_id, const std::
         std::vector<uint32_t> page_ids(n), slot_ids(n), seq_lens(n), q_pos(n), pt_off(n + 1, 0), pt_flat;
         std::vector<RequestSlot> slots(n);
         PageCopies copies;   // of a shared last page, made at once: at most one for a prompt
-        auto finish_copies = [&] { return copies.empty() || (copy_shared_pages(copies) && mlc_pass_flush(ctx) == MLC_OK); };
+        auto finish_copies = [&] {
+            return copies.empty() || (copy_shared_pages(copies, {req.page_state.get()}) && mlc_pass_flush(ctx) == MLC_OK);
+        };
         for (size_t i = 0; i < n; ++i) {
             auto loc = req.page_state->extend_one_token(*ex.pool_, &copies);
             if (!loc) {
@@ -581,7 +591,9 @@ std::vector<float> BatchedWalker::prefill(uint32_t request_id, const std::vector
     std::vector<uint32_t> page_ids(n), slot_ids(n);
     std::vector<RequestSlot> slots(n);
     PageCopies copies;
-    auto finish_copies = [&] { return copies.empty() || (copy_shared_pages(copies) && mlc_pass_flush(ctx) == MLC_OK); };
+    auto finish_copies = [&] {
+        return copies.empty() || (copy_shared_pages(copies, {req.page_state.get()}) && mlc_pass_flush(ctx) == MLC_OK);
+    };
     for (size_t i = 0; i < n; ++i) {
         auto loc = req.page_state->extend_one_token(*ex.pool_, &copies);
         if (!loc) {

@@ -47,8 +47,8 @@ private:
                            bool rows_per_request_only, uint32_t* greedy_host,
                            const PagedAttentionExecutor::BeamStep* beam = nullptr);
     // The copies that a pass's extensions owe (shared pages that it writes into), in every layer's pools, in front of the
-    // pass's kernels. Opens the pass.
-    bool copy_shared_pages(const PageCopies& copies);
+    // pass's kernels. Opens the pass. Where they cannot be made, the requests' tables name the shared pages again.
+    bool copy_shared_pages(const PageCopies& copies, const std::vector<RequestKVState*>& states);
 
     PagedAttentionExecutor& exec_;
     std::vector<float> cos_host_, sin_host_;

@@ -140,6 +140,9 @@ int mlc_kv_state_extend_one_token_owned(mlc_kv_state* s, mlc_page_pool* p, uint3
         return 0;
     }
 }
+int mlc_kv_state_undo_copy(mlc_kv_state* s, mlc_page_pool* p, uint32_t copy_src, uint32_t copy_dst) {
+    return s && p && s->st.undo_copy(p->pool, copy_src, copy_dst) ? 1 : 0;
+}
 int mlc_kv_state_fork(mlc_kv_state* s, const mlc_kv_state* parent, mlc_page_pool* p) {
     if (!s || !parent || !p) return 0;
     try {

@@ -3,6 +3,8 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "ctx.hpp"
 
 namespace mlcb {
@@ -103,6 +105,14 @@ std::optional<std::pair<uint32_t, uint32_t>> RequestKVState::extend_one_token(Pa
         tokens_in_last_page = 0;
     }
     return std::make_pair(page_table.back(), tokens_in_last_page++);
+}
+
+bool RequestKVState::undo_copy(PagePool& pool, uint32_t from, uint32_t to) {
+    const auto at = std::find(page_table.begin(), page_table.end(), to);
+    if (at == page_table.end() || !pool.share(from)) return false;
+    *at = from;
+    pool.release(to);
+    return true;
 }
 
 std::optional<std::pair<uint32_t, uint32_t>> RequestKVState::locate(size_t pos) const {

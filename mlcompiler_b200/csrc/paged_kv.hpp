@@ -64,6 +64,10 @@ struct RequestKVState {
     // The (page, slot) of one more token. A last page with room that other requests own too is replaced by a new one first,
     // and the copy that the device then owes is appended to `copies`; without a list such a page makes the call fail.
     std::optional<std::pair<uint32_t, uint32_t>> extend_one_token(PagePool& pool, PageCopies* copies = nullptr);
+    // Takes such a replacement back where the copy could not be made: the table names `from`, which other requests still own,
+    // again, and `to` goes back to the pool. Rows written into `to` since are lost. False (and unchanged) if the table does
+    // not name `to` or `from` is free.
+    bool undo_copy(PagePool& pool, uint32_t from, uint32_t to);
     // This state becomes a second owner of every page of `parent`. False (and unchanged) if it has pages itself or a page
     // cannot be shared.
     bool fork_from(const RequestKVState& parent, PagePool& pool);

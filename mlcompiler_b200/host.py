@@ -56,6 +56,7 @@ _PROTOTYPES = {
     "mlc_page_pool_owners": (_u32, [_vp, _u32]),
     "mlc_kv_state_fork": (_i, [_vp, _vp, _vp]),
     "mlc_kv_state_extend_one_token_owned": (_i, [_vp, _vp, _u32p, _u32p, _u32p, _u32p]),
+    "mlc_kv_state_undo_copy": (_i, [_vp, _vp, _u32, _u32]),
     "mlc_kv_state_truncate": (_i, [_vp, _vp, _sz]),
     "mlc_executor_run_decode_beams": (_sz, [_vp, C.POINTER(RequestSlotC), _sz, _sz, _fp, C.POINTER(C.c_uint8), _sz, _u32,
                                             _fp, _u32p, _u32p]),
@@ -204,6 +205,10 @@ class RequestKVState:
         p, s, a, b = _u32(0), _u32(0), _u32(0), _u32(0)
         got = lib().mlc_kv_state_extend_one_token_owned(self._h, pool._h, C.byref(p), C.byref(s), C.byref(a), C.byref(b))
         return (p.value, s.value, (a.value, b.value) if got == 2 else None) if got else None
+
+    def undo_copy(self, pool: PagePool, source: int, destination: int) -> bool:
+        """Where the copy could not be made: this state names the shared page again, and the copy's page is free."""
+        return bool(lib().mlc_kv_state_undo_copy(self._h, pool._h, source, destination))
 
     def fork(self, parent: "RequestKVState", pool: PagePool) -> bool:
         """This state, which has no pages, becomes a second owner of all of the parent's."""

@@ -263,3 +263,61 @@ def test_ops_in_one_pass_see_one_another(executor):
     case.sees[0][0, [3, 7, 11]] = True
     want, tol = reference(case, qh, default_scale(case), False)
     assert (np.abs(o2[0].float().cpu().numpy() - want[0]) <= tol[0] + 2.0**-11 * np.abs(want[0]) + 2.0**-25).all()
+
+
+def small_storage(executor, model):
+    """A pool that hands out more pages than the storage holds: a copy into one of those is refused on the host."""
+    pool = PagePool(8)
+    storage = PagedKVStorage(executor, 3, model.n_layers, P, model.kv_heads, model.head_dim, 2)
+    assert storage.initialize()
+    ex = PagedAttentionExecutor(executor, model.num_heads, model.kv_heads, model.head_dim, model.n_layers, 0)
+    ex.attach_page_pool(pool, P)
+    ex.attach_paged_storage(storage)
+    assert ex.attach_model(model.to_device())
+    return pool, storage, ex
+
+
+def test_a_pass_whose_copies_fail_leaves_the_shared_page_where_it_was(executor, model):
+    pool, storage, ex = small_storage(executor, model)
+    tokens = list(range(20))
+    ex.run_prefill(0, tokens)
+    taken = [pool.allocate(), pool.allocate()]          # the next page is the storage's fourth
+    for r in (1, 2):
+        assert ex.fork_request(0, r)
+    out = ex.run_decode([(r, 7, 20) for r in (1, 2)])
+    assert not any(ok for _, ok, _ in out)
+    assert [ex.page_state(r)[0] for r in (0, 1, 2)] == [[0]] * 3
+    assert pool.owners(0) == 3 and pool.pages_in_use() == 3
+    for page in taken:
+        assert pool.release(page)
+    for r in (1, 2):
+        assert ex.truncate_request(r, 20)
+    out = ex.run_decode([(r, 7, 20) for r in (1, 2)])
+    got = [l.copy() for _, ok, l in out if ok]
+    assert len(got) == 2
+    for r in (0, 1, 2):
+        ex.release_request(r)
+    assert pool.pages_in_use() == 0
+    ex.run_prefill(5, tokens)
+    want = ex.run_decode([(5, 7, 20)])[0][2]
+    for g in got:
+        close(g, want)
+
+
+@pytest.mark.parametrize("reference_order", [False, True])
+def test_a_prompt_whose_copy_fails_leaves_the_shared_page_where_it_was(executor, model, reference_order):
+    pool, storage, ex = small_storage(executor, model)
+    ex.set_call_order(reference_order)
+    tokens, tail = list(range(20)), list(range(40, 50))
+    ex.run_prefill(0, tokens)
+    taken = [pool.allocate(), pool.allocate()]
+    assert ex.fork_request(0, 1)
+    assert len(ex.run_prefill(1, tail)) == 0
+    assert ex.page_state(1)[0] == [0] and pool.owners(0) == 2 and pool.pages_in_use() == 3
+    for page in taken:
+        assert pool.release(page)
+    assert ex.truncate_request(1, 20)
+    got = ex.run_prefill(1, tail).copy()
+    for r in (0, 1):
+        ex.release_request(r)
+    close(got, ex.run_prefill(5, tokens + tail))

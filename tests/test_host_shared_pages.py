@@ -135,3 +135,18 @@ def test_a_free_page_is_not_released_again():
     assert pool.pages_in_use() == 1 and pool.pages_free() == 3 and pool.owners(b) == 1
     got = [pool.allocate() for _ in range(3)]
     assert sorted(got + [b]) == [0, 1, 2, 3] and pool.allocate() is None
+
+
+def test_a_copy_that_could_not_be_made_is_taken_back():
+    pool = PagePool(6)
+    parent = filled(pool, 6)                           # pages 0, 1; two tokens in page 1
+    child = RequestKVState(4, 1)
+    assert child.fork(parent, pool)
+    page, slot, copy = child.extend_one_token_owned(pool)
+    assert (page, slot, copy) == (2, 2, (1, 2))
+    assert not child.undo_copy(pool, 1, 3) and not child.undo_copy(pool, 5, 2)     # not its page; a free page
+    assert child.page_table == [0, 2] and pool.owners(2) == 1
+    assert child.undo_copy(pool, 1, 2)
+    assert child.page_table == [0, 1] and [pool.owners(p) for p in range(3)] == [2, 2, 0]
+    assert child.total_tokens() == 7 and child.truncate(pool, 6)
+    assert child.extend_one_token_owned(pool) == (2, 2, (1, 2))

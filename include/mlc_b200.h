@@ -534,7 +534,8 @@ int mlc_encode_paged_prefill_attention(mlc_ctx* ctx, const void* q, const void* 
  * lies in rows that a token does not see - other branches, slots behind the last token - has no
  * effect on it, infinities and NaN included.
  *   q, o          device [sum_r draft_lens[r], num_heads, head_dim], request after request, fp16 or
- *                 fp32 per q_dtype / o_dtype; they must not overlap (MLC_ERR_INVALID_ARG)
+ *                 fp32 per q_dtype / o_dtype; they must not overlap (MLC_ERR_INVALID_ARG). NULL is
+ *                 allowed where no request has a drafted token
  *   tree_mask     host u32 [sum_r draft_lens[r], mask_words]: bit j of row i (word j / 32, bit
  *                 j % 32) set = drafted token i sees drafted token j of its request. A tree sets a
  *                 token's own bit and its ancestors'. Bits at or above draft_lens[r] are ignored;

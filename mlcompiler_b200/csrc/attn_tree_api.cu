@@ -152,8 +152,9 @@ int check_tables(TreeShape& s, const TreeTables& t, size_t n_flat, std::string* 
     return MLC_OK;
 }
 
-int check_call(mlc_ctx* ctx, const TreeArgs& a) {
-    if (!a.q || !a.k_pages || !a.v_pages || !a.o) return ctx->fail(MLC_ERR_INVALID_ARG, "null buffer");
+// Without drafted tokens there is nothing to read or write: q and o may be null then.
+int check_call(mlc_ctx* ctx, const TreeArgs& a, bool rows) {
+    if ((rows && (!a.q || !a.o)) || !a.k_pages || !a.v_pages) return ctx->fail(MLC_ERR_INVALID_ARG, "null buffer");
     if ((a.q_dtype != MLC_F32 && a.q_dtype != MLC_F16) || (a.o_dtype != MLC_F32 && a.o_dtype != MLC_F16))
         return ctx->fail(MLC_ERR_INVALID_ARG, "q / o dtype must be MLC_F16 or MLC_F32");
     if (!aligned_to(a.q, a.q_dtype == MLC_F32 ? 4 : 2) || !aligned_to(a.o, a.o_dtype == MLC_F32 ? 4 : 2) || !aligned_to(a.k_pages, 2) ||
@@ -190,11 +191,11 @@ int prepare_work(mlc_ctx* ctx, const TreeShape& s, const TreeTables& t, TreeWork
 // One call with host tables: the image goes through the context's staging area.
 int tree_impl(mlc_ctx* ctx, bool sync, const TreeArgs& a, TreeShape s, const TreeTables& t, size_t n_flat) {
     if (!ctx) return MLC_ERR_INVALID_ARG;
-    int st = check_call(ctx, a);
-    if (st != MLC_OK) return st;
     s.capacity = resolve_capacity(ctx, a.k_pages, s.capacity, s.P * s.KVH * s.D * 2);
     std::string why;
-    if ((st = check_tables(s, t, n_flat, &why)) != MLC_OK) return ctx->fail(st, "%s", why.c_str());
+    int st = check_tables(s, t, n_flat, &why);
+    if (st != MLC_OK) return ctx->fail(st, "%s", why.c_str());
+    if ((st = check_call(ctx, a, s.tokens > 0)) != MLC_OK) return st;
     if (!sync && !ctx->pass_open) return ctx->fail(MLC_ERR_NO_OPEN_PASS, "encode without an open pass");
     if (ctx->capturing) return ctx->fail(MLC_ERR_UNSUPPORTED, "host tables inside a graph capture: use a plan");
     if (s.tokens == 0) return MLC_OK;
@@ -359,7 +360,7 @@ int mlc_encode_paged_tree_attention_planned(mlc_ctx* ctx, const mlc_tree_plan* p
     if (!ctx->pass_open) return ctx->fail(MLC_ERR_NO_OPEN_PASS, "encode without an open pass");
     if (!plan->ready) return ctx->fail(MLC_ERR_INVALID_ARG, "the plan lost its tables in a failed update");
     const TreeArgs a{q, k_pages, v_pages, o, scale, q_dtype, o_dtype};
-    const int st = check_call(ctx, a);
+    const int st = check_call(ctx, a, plan->shape.tokens > 0);
     if (st != MLC_OK) return st;
     DeviceGuard guard(ctx->device);
     if (ctx->capturing) plan->captured = true;

@@ -442,3 +442,22 @@ def test_sizes_beyond_the_kernels_types_are_refused(ex):
         else:
             assert not ex.runPagedTreeAttention(dev.q, dev.k, dev.v, dev.o, flat, off, prefix, draft, mask, 1, 4, 2, 64, P, 0.0, F16, F16,
                                                 case.capacity) and ex.last_status == 5
+
+
+def test_a_pass_without_any_drafted_token(ex):
+    """No request has one: there is nothing to read or write, and empty tensors have no address."""
+    import torch
+    case = TreeCase(79, [70, 3], [0, 0], 4, 2, 64)
+    dev = OnDevice(case)
+    empty = torch.zeros((0, 4, 64), dtype=torch.float16, device="cuda")
+    assert empty.data_ptr() == 0
+    args = (*case.tables(), 2, 4, 2, 64, 64, 0.0, F16, F16, case.capacity)
+    assert ex.runPagedTreeAttention(empty, dev.k, dev.v, empty, *args), ex.last_error()
+    plan = plan_for(ex, case)
+    ex.beginForwardPassCB()
+    assert ex.encodePagedTreeAttention(empty, dev.k, dev.v, empty, *args), ex.last_error()
+    assert ex.encodePagedTreeAttentionPlanned(plan, empty, dev.k, dev.v, empty), ex.last_error()
+    assert not ex.encodePagedTreeAttentionPlanned(plan, empty, None, dev.v, empty) and ex.last_status == 1
+    assert ex.flushForwardPassCB()
+    dev.result(case)
+    plan.destroy()

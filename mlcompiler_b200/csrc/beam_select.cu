@@ -13,8 +13,9 @@
 // largest at the last clean-up: on real logits few pass it after the first step, and a step in which none does costs one
 // vote. Warps work on their own: 512 rows of 128000, a quarter of them finished, take 59 us (the read
 // of all of them 40); with a CTA per 8192 logits and its five barriers it was 180, with the next step in registers 64.
-// The comparison between beams needs the differences of nearly equal sums: a lane's sum over a step is taken in fp32,
-// what joins the segments and the scores in fp64.
+// The comparison between beams needs the differences of nearly equal sums: a lane's sum over a step, and the warp's over its
+// lanes, are taken in fp32, a lane's steps are added with what their rounding leaves carried along, and what joins the segments
+// and the scores is fp64.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -294,8 +295,10 @@ __device__ __forceinline__ float four_maxima(const float (&x)[16], float (&quart
     for (int j = 0; j < 4; ++j) quarter[j] = fmaxf(max3(x[4 * j], x[4 * j + 1], x[4 * j + 2]), x[4 * j + 3]);
     return fmaxf(max3(quarter[0], quarter[1], quarter[2]), quarter[3]);
 }
-// Sum of the exponentials of 16 logits, the largest of which is `top`, on top of s, relative to the running maximum m.
-__device__ __forceinline__ void add_step(const float (&x)[16], float top, float& m, float& s) {
+// Sum of the exponentials of 16 logits, the largest of which is `top`, on top of s, relative to the running maximum m. `left` is what
+// the additions before have rounded off (Kahan's summation): a step may be smaller than the sum's last bit for hundreds of steps. 512
+// rows of 128000 take 59.3 us so, 60.5 with the sum in fp64, 59.0 without either.
+__device__ __forceinline__ void add_step(const float (&x)[16], float top, float& m, float& s, float& left) {
     const float both = fmaxf(m, top), ref = both == -INFINITY ? 0.f : both;
     const float2 minus = make_float2(-ref, -ref), log2e = make_float2(kLog2e, kLog2e);
     float2 t[2] = {};
@@ -305,7 +308,10 @@ __device__ __forceinline__ void add_step(const float (&x)[16], float top, float&
         t[i & 1] = add2(t[i & 1], make_float2(ex2(d.x), ex2(d.y)));
     }
     t[0] = add2(t[0], t[1]);
-    s = s * exp_diff(m, ref) + (t[0].x + t[0].y);
+    const float scale = exp_diff(m, ref), before = s * scale;
+    const float add = left * scale + (t[0].x + t[0].y);
+    s = before + add;
+    left = add - (s - before);
     m = both;
 }
 
@@ -350,7 +356,7 @@ __device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kSte
             if (step * static_cast<int>(kStep / 4) + static_cast<int>(lane) + 32 * j >= vecs)
                 x[4 * j] = x[4 * j + 1] = x[4 * j + 2] = x[4 * j + 3] = -INFINITY;
     };
-    float m = -INFINITY, s = 0.f, threshold = kLowest;   // (at least the lowest number, so that -inf never passes)
+    float m = -INFINITY, s = 0.f, left = 0.f, threshold = kLowest;   // (at least the lowest number, so that -inf never passes)
     uint64_t lowest = 0;    // once n_select keys are listed: the n_select-th
     uint32_t n = 0;
     auto clean_up = [&] {
@@ -386,7 +392,7 @@ __device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kSte
         drop_behind(step, x);
         float quarter[4];
         const float top = four_maxima(x, quarter);
-        add_step(x, top, m, s);
+        add_step(x, top, m, s, left);
         if (step == 0) {   // 64 disjoint parts: at least n_select logits reach the n_select-th largest of their maxima
             // (a part of NaN alone counts as -inf: NaN is never above anything, and the lanes would not agree on a threshold)
             part[lane] = max3(quarter[0], quarter[1], -INFINITY);
@@ -435,6 +441,7 @@ __device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kSte
     if (__any_sync(0xffffffffu, !(s == s))) {   // NaN among the logits counts as -inf (a sum that +inf spoils stays NaN)
         m = edge > -INFINITY ? edge : -INFINITY;
         s = edge > -INFINITY ? exp_diff(edge, edge) : 0.f;
+        left = 0.f;
 #pragma unroll 1
         for (int step = 0; step < steps; ++step) {
             float x[16];
@@ -444,13 +451,13 @@ __device__ __forceinline__ void segment(const BeamParams& p, float4 (*ring)[kSte
             for (int i = 0; i < 16; ++i)
                 if (!(x[i] == x[i])) x[i] = -INFINITY;
             float quarter[4];
-            add_step(x, four_maxima(x, quarter), m, s);
+            add_step(x, four_maxima(x, quarter), m, s, left);
         }
     }
     float top = m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    s = m > -INFINITY ? s * exp_diff(m, top) : 0.f;
+    s = m > -INFINITY ? (s + left) * exp_diff(m, top) : 0.f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     n = shorten(list, n, p.n_select, lane);

@@ -311,3 +311,21 @@ def test_rows_of_mostly_nan(ex, n, V):
     check(run(ex, x, cum, None, n), reference(x, cum, None, n, 0))
     cum = -np.arange(len(rows), dtype=np.float32).reshape(-1, 2) * 0.015625
     check(run(ex, x, cum, None, n), reference(x, cum, None, n, 0))
+
+
+def test_small_exponentials_add_up_beside_a_large_one(ex):
+    """One likely token per row, the others so far below that a lane's 16 of a step do not reach the last bit of an fp32 sum: over 196
+    steps they make 1e-5. (Enough rows that a row is one segment.)"""
+    import torch
+    G, B, V = 64, 64, 100001
+    x = torch.full((G * B, V), -19.5, device="cuda")
+    x[:, 0] = 0.0
+    cum = -(np.arange(G * B).reshape(G, B) % 64).astype(np.float32)
+    dev = [torch.from_numpy(cum).cuda(), torch.zeros((G, 3), device="cuda")] + [torch.zeros((G, 3), dtype=torch.int32, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    ex.beginForwardPassCB()
+    assert ex.encodeBeamSelect(x, dev[0], None, G, B, V, 0, 3, 0, *dev[1:]), ex.last_error()
+    assert ex.flushForwardPassCB(), ex.last_error()
+    scores = np.tile(np.array([0.0, -1.0, -2.0]) - np.log1p((V - 1) * np.exp(-19.5)), (G, 1))
+    check([dev[1].cpu().numpy()] + [t.cpu().numpy().view(np.uint32) for t in dev[2:]],
+          (scores, np.tile(np.arange(3, dtype=np.uint32), (G, 1)), np.zeros((G, 3), np.uint32)))

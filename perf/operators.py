@@ -17,12 +17,14 @@ _EXECUTORS = {}
 
 
 def _executor():
-    """One context per device with its pass open, as a serving loop keeps it between flushes."""
-    dev = torch.cuda.current_device()
-    if dev not in _EXECUTORS:
+    """One context per device and stream with its pass open, as a serving loop keeps it between flushes. It launches on the stream
+    that the tensors are made and read on. (Torch's default stream has the handle 0, for which a context would make a stream of its
+    own, ordered with nothing; 1 is CUDA's handle of the same default stream.)"""
+    dev, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream or 1
+    if (dev, stream) not in _EXECUTORS:
         from mlcompiler_b200 import Executor
-        _EXECUTORS[dev] = Executor(dev)
-    ex = _EXECUTORS[dev]
+        _EXECUTORS[dev, stream] = Executor(dev, stream=stream)
+    ex = _EXECUTORS[dev, stream]
     if not ex.hasForwardPassCB():
         ex.beginForwardPassCB()
     return ex

@@ -540,7 +540,9 @@ int mlc_encode_paged_prefill_attention(mlc_ctx* ctx, const void* q, const void* 
  *                 j % 32) set = drafted token i sees drafted token j of its request. A tree sets a
  *                 token's own bit and its ancestors'. Bits at or above draft_lens[r] are ignored;
  *                 mask_words * 32 must be >= every draft_lens[r].
- *   the other tables, scale, capacity_pages as in mlc_encode_paged_flash_attention;
+ *   the other tables, scale, capacity_pages as in mlc_encode_paged_flash_attention; a plan knows no
+ *   pool to look the capacity up for: made without capacity_pages its page ids are not checked, and
+ *   its calls take the general kernel, which reads the cache once per drafted token and head;
  *   prefix_lens[r] + draft_lens[r] must fit the request's pages. Requests without drafted tokens
  *   are allowed.
  * run_: validates, launches, waits. encode_: asynchronous, needs an open pass. The plan keeps one

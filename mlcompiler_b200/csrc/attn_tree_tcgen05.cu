@@ -351,7 +351,7 @@ paged_tree_tcgen05_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_
     };
 
     // Two fp32 CTAs an SM leave a thread 128 registers at launch, and softmax with both halves of P spills: the other warpgroup
-    // gives it some (the sum stays 2 * 128). 8 requests in fp32, with one reference for all tiles: 20.3 us without, 19.4 with; fp16 does not gain.
+    // gives it some (the sum stays 2 * 128). 8 requests in fp32: 19.5 us without, 18.9 with; fp16 does not gain.
     if constexpr (EXACT && C::ctas == 2) {
         if (warp < 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));

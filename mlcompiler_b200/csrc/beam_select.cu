@@ -12,7 +12,7 @@
 // segment needs no logarithm. The largest logits are kept as a list in shared memory with a threshold, the n_select-th
 // largest at the last clean-up: on real logits few pass it after the first step, and a step in which none does costs one
 // vote. Warps work on their own: 512 rows of 128000, a quarter of them finished, take 59 us (the read
-// of all of them 40); with a CTA per 8192 logits and its five barriers it was 180, with the next step in registers 64.
+// of the others 30); with a CTA per 8192 logits and its five barriers it was 180, with the next step in registers 64.
 // The comparison between beams needs the differences of nearly equal sums: a lane's sum over a step, and the warp's over its
 // lanes, are taken in fp32, a lane's steps are added with what their rounding leaves carried along, and what joins the segments
 // and the scores is fp64.
